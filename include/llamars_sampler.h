@@ -230,6 +230,80 @@ int  lrs_history_append(const uint32_t* d_tokens, const int32_t* d_status, uint3
 int  lrs_remap_tokens(const uint32_t* d_tokens, const int32_t* d_status, uint32_t rows,
                       const uint32_t* d_map, uint32_t map_n, uint32_t* d_out, void* stream);
 
+/* ---- draws from given uniforms ---------------------------------------------------
+ * No counterpart in the reference, whose sampler owns its generator and has no min-p: the
+ * draw of a serving loop that brings its own random numbers (one uniform a row), on logits
+ * of 32 or 16 bits.  Not bit-compatible with lrs_sample_device and not meant to be: here
+ * the definition is over the real numbers, the kernels hold every weight and sum in 64 bits,
+ * and the token is found in vocabulary order.  For row r, x = its logits, M = max x:
+ *   weights  w_i = exp((x_i - M) / temperature), Z = the sum of all w
+ *   order    by x descending, equal x by ascending index
+ *   kept     the shortest of these prefixes of the order: the first top_k elements (0, or
+ *            >= n: off); the elements with w_i >= min_p (0: off); the shortest prefix whose
+ *            weights reach top_p * Z (off unless 0 < top_p < 1; Z is the whole row's, as in
+ *            sampler.rs:135-146).  At least one element is kept; -inf never is
+ *   token    the smallest index i with sum of the kept w_j, j <= i, > u * (their whole sum)
+ *   prob     w_i / (sum of the kept w): the token's probability among the kept ones
+ * temperature <= 0 is greedy: the lowest index of the largest logit, prob 1, kept 1 (the
+ * other parameters and u are not read).
+ * Row status (d_status): LRS_OK; LRS_E_NAN if the row holds a NaN or +inf, or nothing above
+ * -inf; LRS_E_INVALID if temperature is not finite, top_p is NaN, min_p is outside [0, 1] or
+ * u outside [0, 1).  Such a row gets token LRS_TOKEN_NONE, prob 0 and kept 0, and every other
+ * row is drawn.
+ *   d_logits  row r = d_logits + r * ld elements (ld >= n, or 0: every row reads row 0), any
+ *             alignment of the element type; dtype LRS_F32, LRS_BF16 or LRS_F16
+ *   n         1 <= n <= LRS_DRAW_MAX_VOCAB; rows <= LRS_DRAW_MAX_ROWS
+ *   d_probs, d_kept (elements kept), d_status: nullable
+ * Enqueued on `stream` (cudaStream_t of the current device), no host synchronisation.  The
+ * call keeps no state and no working memory: calls may overlap, be captured into graphs and
+ * replayed at once.  Returns LRS_OK, LRS_E_INVALID or LRS_E_CUDA (lrs_last_error(NULL)).  */
+#define LRS_F32  0
+#define LRS_BF16 1
+#define LRS_F16  2
+typedef struct lrs_draw_params {
+    float    temperature;
+    uint32_t top_k;
+    float    top_p;
+    float    min_p;
+} lrs_draw_params;
+#define LRS_DRAW_MAX_VOCAB (1u << 22)
+#define LRS_DRAW_MAX_ROWS  (1u << 24)
+int  lrs_draw_device(const void* d_logits, int dtype, uint32_t rows, uint32_t n, uint64_t ld,
+                     const lrs_draw_params* d_params, const float* d_uniform, uint32_t* d_tokens,
+                     float* d_probs, uint32_t* d_kept, int32_t* d_status, void* stream);
+
+/* ---- language-model head in 8-bit floating point -----------------------------------
+ * The product whose rows the samplers read (model.rs:579-582, 733-737: ops::matmul over the
+ * vocabulary), on e4m3 codes with an f32 scale for each block of 128 columns.
+ * lrs_quantize_rows    activations: row r, columns 128 b .. 128 b + 127 share d_scale[b * ld_scale
+ *                      + r] (block-major, ld_scale >= rows)
+ * lrs_quantize_blocks  weights: rows 128 a .., columns 128 b .. share d_scale[a * ld_scale + b]
+ *                      (ld_scale >= ceil(k / 128))
+ *   Of a block with the largest magnitude m: scale = max(m / 448, 2^-126), code =
+ *   e4m3(x * (1 / scale)), each operation rounded once (codes to nearest even).  A block that
+ *   holds a NaN or an infinity gets a non-finite scale, so that every product with it is NaN
+ *   (and the samplers report LRS_E_NAN).  d_x: dtype LRS_F32, LRS_BF16 or LRS_F16, row r at
+ *   d_x + r * ld_x elements (ld_x >= k, any alignment of the type); d_q: row r at d_q + r *
+ *   ld_q bytes (ld_q >= k); bytes k .. ld_q of a row are left as they were.
+ * lrs_fp8_logits       d_out[r][v] = sum over b of a_scale[b * ld_as + r] * w_scale[v / 128 * ld_ws + b]
+ *                      * (sum over the block's columns of a[r][c] * w[v][c]), r < rows, v < n: the
+ *                      block sums in f32 on the tensor cores, the sum over blocks in f32, rounded
+ *                      once to out_dtype.  d_out: row r at d_out + r * ld_out elements (ld_out >=
+ *                      n, any alignment of the type).  Codes: d_a + r * ld_a and d_w + v * ld_w
+ *                      bytes (>= k), bases and (of more than one row) ld_a, ld_w multiples of 16.
+ * rows, n, k >= 1; rows, n <= 2^24, k <= 2^18 (LRS_E_INVALID otherwise; rows == 0 returns LRS_OK).
+ * Enqueued on `stream` (cudaStream_t of the current device) without host synchronisation; no
+ * state and no working memory is kept.  They return LRS_OK, LRS_E_INVALID or LRS_E_CUDA
+ * (lrs_last_error(NULL)).                                                              */
+int  lrs_quantize_rows(const void* d_x, int dtype, uint32_t rows, uint32_t k, uint64_t ld_x,
+                       uint8_t* d_q, uint64_t ld_q, float* d_scale, uint64_t ld_scale, void* stream);
+int  lrs_quantize_blocks(const void* d_x, int dtype, uint32_t rows, uint32_t k, uint64_t ld_x,
+                         uint8_t* d_q, uint64_t ld_q, float* d_scale, uint64_t ld_scale, void* stream);
+int  lrs_fp8_logits(const uint8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint64_t ld_as,
+                    const uint8_t* d_w, uint64_t ld_w, const float* d_w_scale, uint64_t ld_ws,
+                    uint32_t rows, uint32_t n, uint32_t k, void* d_out, int out_dtype, uint64_t ld_out,
+                    void* stream);
+
 /* ---- single-row drop-in (Sampler API) -------------------------------------------
  * lrs_sampler_new    replaces Sampler::new(seed)               (sampler.rs:33-37)
  * lrs_sampler_sample replaces Sampler::sample(logits, params, recent) (sampler.rs:56)

@@ -21,6 +21,7 @@
 #include "lrs_device.cuh"
 
 #include "lrs_kernels_decl.cuh"
+#include "lrs_ops.cuh"
 
 namespace {
 thread_local std::string g_create_error;
@@ -85,6 +86,20 @@ static int set_err(lrs_ctx* c, int code, const char* fmt, ...) {
         c->err = buf;
     else
         g_create_error = buf;
+    return code;
+}
+
+// Errors of the calls without a context (lrs_ops.cuh): lrs_last_error(NULL) of this thread.
+int lrs_call_error(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    try {
+        g_create_error = buf;
+    } catch (...) {  // (no memory for the message: the status says enough)
+    }
     return code;
 }
 

@@ -19,12 +19,12 @@ GEN = os.path.join(PKG_DIR, "data", "gen_expf_table")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-O3", "-std=c++17", "-lineinfo",
+    "-O3", "-std=c++17", "-lineinfo", "--threads", "0",
     "-Xcompiler", "-fPIC,-O2",
     "-Xptxas", "-warn-spills",
 ]
-SOURCES = ["lrs_kernels.cu", "lrs_api.cu", "lrs_noalloc.cu", "lrs_generate.cu"]
-HEADERS = ["lrs_device.cuh", "lrs_grid.h", "lrs_kernels_decl.cuh", "lrs_stages.cuh"]
+SOURCES = ["lrs_kernels.cu", "lrs_api.cu", "lrs_noalloc.cu", "lrs_generate.cu", "lrs_draw.cu", "lrs_quant.cu", "lrs_head.cu"]
+HEADERS = ["lrs_device.cuh", "lrs_grid.h", "lrs_kernels_decl.cuh", "lrs_stages.cuh", "lrs_ops.cuh"]
 
 
 def _newer(target: str, deps: list[str]) -> bool:

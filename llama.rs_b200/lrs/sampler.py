@@ -39,13 +39,16 @@ ROW_INFO_DTYPE = np.dtype([
     ("reserved", "<u4"),
 ])
 
+# lrs_draw_params: the filters of a draw from given uniforms (BatchSampler.draw_device)
+DRAW_PARAMS_DTYPE = np.dtype([("temperature", "<f4"), ("top_k", "<u4"), ("top_p", "<f4"), ("min_p", "<f4")])
+
 # Every entry point declared in include/llamars_sampler.h.
 EXPORTS = [
     "lrs_create", "lrs_destroy", "lrs_last_error", "lrs_seed_state", "lrs_set_state", "lrs_get_state",
     "lrs_set_params", "lrs_sample", "lrs_sample_device", "lrs_sampler_new", "lrs_sampler_free",
     "lrs_sampler_state", "lrs_sampler_sample", "lrs_sample_device_noalloc", "lrs_assemble_shards",
     "lrs_poll_error", "lrs_noalloc_poll_error", "lrs_test_wait_timeout", "lrs_history_append",
-    "lrs_remap_tokens",
+    "lrs_remap_tokens", "lrs_draw_device", "lrs_quantize_rows", "lrs_quantize_blocks", "lrs_fp8_logits",
 ]
 
 
@@ -99,6 +102,13 @@ def lib() -> ctypes.CDLL:
         L.lrs_history_append.restype = I
         L.lrs_remap_tokens.argtypes = [P, P, U32, P, U32, P, P]
         L.lrs_remap_tokens.restype = I
+        L.lrs_draw_device.argtypes = [P, I, U32, U32, U64, P, P, P, P, P, P, P]
+        L.lrs_draw_device.restype = I
+        for f in (L.lrs_quantize_rows, L.lrs_quantize_blocks):
+            f.argtypes = [P, I, U32, U32, U64, P, U64, P, U64, P]
+            f.restype = I
+        L.lrs_fp8_logits.argtypes = [P, U64, P, U64, P, U64, P, U64, U32, U32, U32, P, I, U64, P]
+        L.lrs_fp8_logits.restype = I
         L.lrs_sampler_new.argtypes = [U64, I]
         L.lrs_sampler_new.restype = P
         L.lrs_sampler_free.argtypes = [P]
@@ -137,6 +147,49 @@ def _check(code: int, ctx=None):
         if code == LRS_E_NAN:
             raise SamplerPanic(code, msg)
         raise SamplerError(code, msg)
+
+
+_dtype_codes = None
+
+
+def dtype_code(t) -> int:
+    """LRS_F32, LRS_BF16 or LRS_F16 of a tensor (SamplerError for any other type)."""
+    global _dtype_codes
+    if _dtype_codes is None:
+        import torch
+        _dtype_codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    code = _dtype_codes.get(t.dtype)
+    if code is None:
+        raise SamplerError(LRS_E_INVALID, f"{t.dtype}: float32, bfloat16 or float16 is needed")
+    return code
+
+
+class _Launch:
+    """The device and stream of a call without a context: checks that the tensors (None: absent) lie
+    on one GPU, makes it the current device while the call is enqueued, and gives the stream's
+    handle (torch's current stream there unless `stream` is given)."""
+    __slots__ = ("stream", "device", "back")
+
+    def __init__(self, stream, *tensors):
+        d = tensors[0].get_device()
+        if d < 0:
+            raise SamplerError(LRS_E_INVALID, "CUDA tensors are needed")
+        for t in tensors:
+            if t is not None and t.get_device() != d:
+                raise SamplerError(LRS_E_INVALID, "the tensors lie on different devices")
+        self.stream, self.device = stream, d
+
+    def __enter__(self):
+        import torch
+        self.back = torch.cuda.current_device()
+        if self.back != self.device:
+            torch.cuda.set_device(self.device)
+        return torch.cuda.current_stream(self.device).cuda_stream if self.stream is None else self.stream
+
+    def __exit__(self, *exc):
+        if self.back != self.device:
+            import torch
+            torch.cuda.set_device(self.back)
 
 
 class Sampler:
@@ -236,6 +289,52 @@ class BatchSampler:
                                        params.data_ptr(), state.data_ptr(), tokens.data_ptr(), ptr(probs),
                                        ptr(status), ptr(info), stream)
         _check(code, self._h)
+
+    @staticmethod
+    def draw_device(logits, params, uniform, tokens, probs=None, kept=None, status=None, n=None, stream=None,
+                    ld=None, rows=None):
+        """Tokens from given uniforms (lrs_draw_device) under temperature, top-k, top-p and min-p:
+        logits (rows, n) float32 / bfloat16 / float16, params rows of DRAW_PARAMS_DTYPE (any 4-byte or
+        byte tensor of them), uniform float32 in [0, 1); tokens, kept and status are int32 tensors,
+        probs float32.  The definition of the kept set and of the draw is the header's.  Async; no
+        working memory and no context, so calls may overlap and be captured."""
+        rows = tokens.numel() if rows is None else rows
+        if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise SamplerError(LRS_E_INVALID, "logits: a 2-d tensor with contiguous rows is needed")
+        n = logits.shape[1] if n is None else n
+        if ld is None:
+            ld = logits.stride(0) if logits.shape[0] > 1 else n if rows <= 1 else 0
+        have = logits.shape[0] if ld else rows
+        if rows > have or n > logits.shape[1] or params.numel() * params.element_size() < 16 * rows:
+            raise SamplerError(LRS_E_INVALID, f"draw_device: the logits or the parameters hold fewer than {rows} rows of {n}")
+        for t in (params, uniform, tokens, probs, kept, status):
+            if t is not None and not t.is_contiguous():
+                raise SamplerError(LRS_E_INVALID, "draw_device: a buffer of a value a row is not contiguous")
+        for t in (uniform, tokens, probs, kept, status):
+            if t is not None and (t.numel() < rows or t.element_size() != 4):
+                raise SamplerError(LRS_E_INVALID, f"draw_device: a buffer holds fewer than {rows} 32-bit values")
+        with _Launch(stream, logits, params, uniform, tokens, probs, kept, status) as s:
+            _check(lib().lrs_draw_device(logits.data_ptr(), dtype_code(logits), rows, n, ld, params.data_ptr(),
+                                         uniform.data_ptr(), tokens.data_ptr(),
+                                         None if probs is None else probs.data_ptr(),
+                                         None if kept is None else kept.data_ptr(),
+                                         None if status is None else status.data_ptr(), s))
+
+    @staticmethod
+    def draw_hidden(head, hidden, params, uniform, tokens, probs=None, kept=None, status=None, dtype=None):
+        """A decode step's end: the head's logits (LmHead.logits, in `dtype`, float32 by default) of the
+        hidden states, and a token a row from them (draw_device).  On torch's current stream."""
+        logits = head.logits(hidden, dtype=dtype)
+        BatchSampler.draw_device(logits, params, uniform, tokens, probs=probs, kept=kept, status=status,
+                                 rows=hidden.shape[0])
+        return logits
+
+    def sample_hidden(self, head, hidden, params, state, tokens, hist=None, hist_len=None, probs=None, status=None):
+        """The same with the exact sampler: the head's logits of the hidden states, then sample_device."""
+        logits = head.logits(hidden)
+        self.sample_device(logits, params, state, tokens, hist=hist, hist_len=hist_len, probs=probs, status=status,
+                           rows=hidden.shape[0])
+        return logits
 
     @staticmethod
     def history_append(tokens, hist, hist_len, status=None, eos=None, keep=None, stream=None, rows=None):

@@ -208,5 +208,14 @@ class VocabShardedSampler:
         self.sample_owned(params, state, tokens, hist=hist, hist_len=hist_len, probs=probs, status=status,
                           stream=stream)
 
+    def sample_hidden(self, head, hidden, params, state, tokens, hist=None, hist_len=None, probs=None,
+                      status=None) -> None:
+        """A tensor-parallel head in front of sample(): `head` (LmHead) holds this rank's vocab / world
+        rows of the weights, `hidden` (rows, k) every row's hidden states.  On torch's current stream."""
+        if head.vocab != self.shard_n or hidden.shape[0] != self.rows:
+            raise ValueError(f"a head of {self.shard_n} tokens and {self.rows} hidden states are needed")
+        self.sample(head.logits(hidden), params, state, tokens, hist=hist, hist_len=hist_len, probs=probs,
+                    status=status)
+
     def close(self) -> None:
         self.bs.close()

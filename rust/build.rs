@@ -29,10 +29,12 @@ fn main() {
     let include = manifest.join("../include");
     let out = PathBuf::from(env::var("OUT_DIR").unwrap());
     let nvcc = env::var("NVCC").unwrap_or_else(|_| "/usr/local/cuda/bin/nvcc".into());
-    let sources = ["lrs_kernels.cu", "lrs_api.cu", "lrs_noalloc.cu"];
+    let sources = [
+        "lrs_kernels.cu", "lrs_api.cu", "lrs_noalloc.cu", "lrs_generate.cu", "lrs_draw.cu", "lrs_quant.cu", "lrs_head.cu",
+    ];
     for f in sources
         .iter()
-        .chain(["lrs_device.cuh", "lrs_grid.h", "lrs_kernels_decl.cuh", "lrs_stages.cuh", "gen_expf_table.c"].iter())
+        .chain(["lrs_device.cuh", "lrs_grid.h", "lrs_kernels_decl.cuh", "lrs_stages.cuh", "lrs_ops.cuh", "gen_expf_table.c"].iter())
     {
         println!("cargo:rerun-if-changed={}", csrc.join(f).display());
     }

@@ -5,6 +5,7 @@
 //! Not compiled in this repository's build image (it has no Rust toolchain); the ABI this
 //! crate declares (src/ffi.rs) is checked by tests/csrc/rust_abi.c in the CPU test suite.
 pub mod ffi;
+pub mod ops;
 pub mod sampler;
 pub mod stream;
 

@@ -67,7 +67,7 @@ impl fmt::Display for SamplerError {
 
 impl std::error::Error for SamplerError {}
 
-fn check(code: i32, ctx: *const ffi::lrs_ctx) -> Result<(), SamplerError> {
+pub(crate) fn check(code: i32, ctx: *const ffi::lrs_ctx) -> Result<(), SamplerError> {
     if code == ffi::LRS_OK {
         return Ok(());
     }
