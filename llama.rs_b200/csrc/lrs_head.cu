@@ -1,16 +1,20 @@
 // lrs_head.cu — the language-model head's product in 8-bit floating point (sm_100a):
 //   out[r][v] = sum over blocks b of sa[b][r] sw[v / 128][b] (sum over the block of a[r][c] w[v][c])
 //
-// The weights are the tensor core's 128-row operand and the hidden states its other one, so a few
-// rows (a decode step) cost a narrow instruction and not a padded one, and a warp's 32 lanes hold 32
-// consecutive logits of one row.  A block of 128 columns is one step: four tcgen05.mma (kind
-// f8f6f4, K = 32) into TMEM from zero, read back by the epilogue warps and added to f32 registers
-// with the block's scale, while the tensor core fills the other TMEM buffer.
-//
-// Persistent CTAs of twelve warps: 0 issues the TMA copies of both operands (128-byte swizzle, a
-// ring of stages), 1 issues the MMAs, 2 brings the scales of a step (4-byte asynchronous copies: any
-// alignment), 4-11 are the epilogue, a quarter of the lanes and half of the columns each.  Tiles walk
-// the row tiles first, so that the CTAs share the weights they stream in L2.
+// A block of 128 columns is one step: four tcgen05.mma (kind f8f6f4, K = 32) into TMEM from zero, read
+// back by the epilogue warps and added to f32 registers with the block's scales, while the tensor core
+// fills another TMEM buffer.  Persistent CTAs of twenty warps: 0 issues the TMA copies of both operands
+// (128-byte swizzle, a ring of stages), 1 issues the MMAs, 4-19 are the epilogue.  Tiles walk the row
+// tiles first, so that the CTAs share the weights they stream in L2.  Two forms:
+//   narrow  up to 64 rows (a decode step; bound by the weights' bytes): the weights are the tensor core's
+//           128-row operand, so a few rows cost a narrow instruction and not a padded one, and a warp's
+//           lanes are consecutive logits of one row.  A row is a TMEM column there, its scale the same
+//           for a whole warp: warp 2 brings them to shared memory (4-byte asynchronous copies: any
+//           alignment), from where a thread reads one for each of its 16 columns.
+//   wide    more rows: 128 rows x 256 vocabulary entries.  A row is a TMEM lane, so a thread has one
+//           row scale and one weight scale a step and adds with a single factor (with the rows as
+//           columns the scales' shared-memory reads and products took three times the MMAs' time); the
+//           logits go out through shared memory, 64 bytes of a row at a time.
 #include <cuda.h>
 
 #include "lrs_ops.cuh"
@@ -20,10 +24,9 @@ namespace {
 using namespace lrs;
 
 constexpr uint32_t kBlock = 128;      // columns a scale covers, and columns of a step
-constexpr uint32_t kTileV = 128;      // vocabulary entries of a tile
-constexpr uint32_t kMaxTileR = 256;   // rows of a tile at most
-constexpr uint32_t kThreads = 384;
-constexpr uint32_t kEpilogueWarps = 8;
+constexpr uint32_t kNarrowRows = 64;  // rows of the narrow form at most
+constexpr uint32_t kThreads = 640;
+constexpr uint32_t kMaxBuffers = 8;   // TMEM accumulators
 constexpr uint32_t kScaleStages = 8;
 constexpr uint32_t kMaxStages = 10;
 constexpr long long kWaitCycles = 1ll << 32;  // about 2 s: no wait of a sound launch comes near it
@@ -50,6 +53,24 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return done != 0;
 }
+// Position in a ring of barriers.
+struct Ring {
+    uint32_t at = 0, turn = 0;
+    __device__ __forceinline__ void next(uint32_t size) {
+        if (++at == size) at = 0, turn ^= 1;
+    }
+};
+
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 // Waits for a phase; false when the bound has passed or another warp has given up.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* lost) {
     if (bar_try(bar, parity)) return true;
@@ -60,6 +81,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     } while (clock64() - t0 < kWaitCycles);
     *lost = 1;
     return false;
+}
+// The same for a whole warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* lost) {
+    return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, lost));
 }
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
@@ -85,15 +110,6 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[8]) {
-    uint32_t r[8];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(addr)
-                 : "memory");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-}
 __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) {
     uint32_t r[16];
     asm volatile(
@@ -108,48 +124,38 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) {
 }
 
 // Completes the loads: the registers pass through, so that nothing reads them earlier.
-__device__ __forceinline__ void tmem_wait(float (&v)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])::"memory");
-}
 __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
                    "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 struct Args {
     const float* sa;
     const float* sw;
     void* out;
     uint64_t ld_as, ld_ws, ld_out;
-    uint32_t rows, n, blocks;        // blocks of 128 columns
-    uint32_t tile_r, row_tiles;      // rows of a tile (16, or a multiple of 32), tiles over the rows
-    uint32_t tiles;                  // all of them
-    uint32_t stages, tmem_cols;
+    uint32_t rows, n, blocks;          // blocks of 128 columns
+    uint32_t tile_r, tile_v;           // rows and vocabulary entries of a tile
+    uint32_t row_tiles, tiles;         // tiles over the rows, all of them
+    uint32_t first_bytes, stage_bytes; // of the 128-row operand, of a stage
+    uint32_t stages, buffers;          // of shared memory, of TMEM
+    uint32_t columns, tmem_columns;    // of a buffer, allocated
 };
 
 struct Barriers {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t sfull[kScaleStages], sempty[kScaleStages];
-    uint64_t tfull[2], tempty[2];
+    uint64_t tfull[kMaxBuffers], tempty[kMaxBuffers];
     uint64_t drain;
     uint32_t tmem;
     uint32_t lost;
 };
 
-// HALF: columns of an epilogue warp at most (half of tile_r); CHUNK: columns of one TMEM load.
-template <typename T, int HALF, int CHUNK>
-__global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant__ CUtensorMap map_w,
-                                                           const __grid_constant__ CUtensorMap map_a, const Args g) {
-    extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ Barriers bars;
-    __shared__ __align__(16) float scales[kScaleStages][kMaxTileR + 4];
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t base = (smem_of(smem) + 1023u) & ~1023u;
-    const uint32_t stage_bytes = kTileV * kBlock + g.tile_r * kBlock;
-    volatile uint32_t* lost = &bars.lost;
-
+// Barriers and TMEM of a CTA; `releases` arrivals free a TMEM buffer (and a stage of scales).
+__device__ __forceinline__ uint32_t set_up(const Args& g, Barriers& bars, uint32_t releases) {
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < g.stages; ++s) {
             bar_init(smem_of(&bars.full[s]), 1);
@@ -157,158 +163,293 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         }
         for (uint32_t s = 0; s < kScaleStages; ++s) {
             bar_init(smem_of(&bars.sfull[s]), 32);
-            bar_init(smem_of(&bars.sempty[s]), kEpilogueWarps);
+            bar_init(smem_of(&bars.sempty[s]), releases);
         }
-        for (uint32_t s = 0; s < 2; ++s) {
+        for (uint32_t s = 0; s < g.buffers; ++s) {
             bar_init(smem_of(&bars.tfull[s]), 1);
-            bar_init(smem_of(&bars.tempty[s]), kEpilogueWarps);
+            bar_init(smem_of(&bars.tempty[s]), releases);
         }
         bar_init(smem_of(&bars.drain), 1);
         bars.lost = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
+    if (threadIdx.x / 32 == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&bars.tmem)),
-                     "r"(g.tmem_cols)
+                     "r"(g.tmem_columns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    tmem_fence_before();
     __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *(volatile uint32_t*)&bars.tmem;
+    tmem_fence_after();
+    return *(volatile uint32_t*)&bars.tmem;
+}
+
+__device__ __forceinline__ void tear_down(const Args& g, uint32_t tmem) {
+    tmem_fence_before();
+    __syncthreads();
+    if (threadIdx.x / 32 == 1) {
+        __syncwarp();
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_columns) : "memory");
+    }
+}
+
+// Warp 0: the copies of both operands of every step; the 128-row operand comes first in a stage.
+__device__ __forceinline__ void copy_warp(const Args& g, Barriers& bars, uint32_t base, const CUtensorMap* first,
+                                          const CUtensorMap* second, bool weights_first) {
+    volatile uint32_t* lost = &bars.lost;
+    Ring ring;
+    uint32_t issued = 0;
+    bool ok = true;
+    for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
+        const uint32_t r0 = t % g.row_tiles * g.tile_r, v0 = t / g.row_tiles * g.tile_v;
+        const uint32_t y0 = weights_first ? v0 : r0, y1 = weights_first ? r0 : v0;
+        for (uint32_t b = 0; b < g.blocks; ++b) {
+            ok = warp_wait(smem_of(&bars.empty[ring.at]), ring.turn ^ 1, lost);
+            if (!ok) break;
+            if (elect()) {
+                const uint32_t bar = smem_of(&bars.full[ring.at]), at = base + ring.at * g.stage_bytes;
+                bar_expect(bar, g.stage_bytes);
+                tma_load(at, first, b * kBlock, y0, bar);
+                tma_load(at + g.first_bytes, second, b * kBlock, y1, bar);
+            }
+            __syncwarp();
+            ring.next(g.stages);
+            ++issued;
+        }
+    }
+    if (!ok) {  // copies that a warp which gave up did not wait for land before the CTA ends
+        for (uint32_t j = issued > g.stages ? issued - g.stages : 0; j < issued; ++j) {
+            const long long t0 = clock64();
+            while (!bar_try(smem_of(&bars.full[j % g.stages]), j / g.stages & 1) && clock64() - t0 < kWaitCycles) {
+            }
+        }
+    }
+}
+
+// Warp 1: the MMAs of every step, 128 x `columns` into the next TMEM buffer.
+__device__ __forceinline__ void mma_warp(const Args& g, Barriers& bars, uint32_t base, uint32_t tmem) {
+    volatile uint32_t* lost = &bars.lost;
+    const uint32_t idesc = 1u << 4 | g.columns / 8 << 17 | 128 / 16 << 24;  // f32 += e4m3 x e4m3, both K-major
+    Ring ring, buffer;
+    bool ok = true;
+    for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
+        for (uint32_t b = 0; b < g.blocks; ++b) {
+            ok = warp_wait(smem_of(&bars.tempty[buffer.at]), buffer.turn ^ 1, lost) &&
+                 warp_wait(smem_of(&bars.full[ring.at]), ring.turn, lost);
+            if (!ok) break;
+            tmem_fence_after();
+            if (elect()) {
+                const uint32_t at = base + ring.at * g.stage_bytes, d = tmem + buffer.at * g.columns;
+                const uint64_t da = operand(at), db = operand(at + g.first_bytes);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) mma(d, da + 2 * j, db + 2 * j, idesc, j > 0);
+                mma_commit(smem_of(&bars.empty[ring.at]));
+                mma_commit(smem_of(&bars.tfull[buffer.at]));
+            }
+            __syncwarp();
+            ring.next(g.stages);
+            buffer.next(g.buffers);
+        }
+    }
+    // every MMA has ended before the TMEM goes back
+    if (elect()) mma_commit(smem_of(&bars.drain));
+    __syncwarp();
+    const long long t0 = clock64();
+    while (!bar_try(smem_of(&bars.drain), 0) && clock64() - t0 < kWaitCycles) {
+    }
+    __syncwarp();
+}
+
+constexpr float kLost = __builtin_nanf("");  // what a wait that ran out leaves: the samplers report it
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                             const __grid_constant__ CUtensorMap map_a, const Args g) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ Barriers bars;
+    __shared__ __align__(16) float scales[kScaleStages][kNarrowRows + 4];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, groups = g.tile_r / 16;
+    const uint32_t base = (smem_of(smem) + 1023u) & ~1023u;
+    volatile uint32_t* lost = &bars.lost;
+    const uint32_t tmem = set_up(g, bars, 4 * groups);
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
-                const uint32_t r0 = t % g.row_tiles * g.tile_r, v0 = t / g.row_tiles * kTileV;
-                for (uint32_t b = 0; b < g.blocks; ++b, ++it) {
-                    const uint32_t s = it % g.stages;
-                    ok = bar_wait(smem_of(&bars.empty[s]), (it / g.stages & 1) ^ 1, lost);
-                    if (!ok) break;
-                    const uint32_t bar = smem_of(&bars.full[s]), at = base + s * stage_bytes;
-                    bar_expect(bar, stage_bytes);
-                    tma_load(at, &map_w, b * kBlock, v0, bar);
-                    tma_load(at + kTileV * kBlock, &map_a, b * kBlock, r0, bar);
-                }
-            }
-            // (copies that a warp which gave up did not wait for land before the CTA ends)
-            if (!ok)
-                for (uint32_t j = it > g.stages ? it - g.stages : 0; j < it; ++j) {
-                    const long long t0 = clock64();
-                    while (!bar_try(smem_of(&bars.full[j % g.stages]), j / g.stages & 1) && clock64() - t0 < kWaitCycles) {
-                    }
-                }
-        }
+        copy_warp(g, bars, base, &map_w, &map_a, true);
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = 1u << 4 | g.tile_r / 8 << 17 | kTileV / 16 << 24;  // f32 += e4m3 x e4m3, both K-major
-            uint32_t it = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
-                for (uint32_t b = 0; b < g.blocks; ++b, ++it) {
-                    const uint32_t s = it % g.stages, buf = it & 1;
-                    ok = bar_wait(smem_of(&bars.tempty[buf]), (it / 2 & 1) ^ 1, lost) &&
-                         bar_wait(smem_of(&bars.full[s]), it / g.stages & 1, lost);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = base + s * stage_bytes, d = tmem + buf * (g.tmem_cols / 2);
-                    const uint64_t da = operand(at), db = operand(at + kTileV * kBlock);
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) mma(d, da + 2 * j, db + 2 * j, idesc, j > 0);
-                    mma_commit(smem_of(&bars.empty[s]));
-                    mma_commit(smem_of(&bars.tfull[buf]));
-                }
-            }
-            // every MMA has ended before the TMEM goes back
-            mma_commit(smem_of(&bars.drain));
-            const long long t0 = clock64();
-            while (!bar_try(smem_of(&bars.drain), 0) && clock64() - t0 < kWaitCycles) {
-            }
-        }
-        __syncwarp();
+        mma_warp(g, bars, base, tmem);
     } else if (warp == 2) {
-        uint32_t it = 0;
+        Ring ring;
         bool ok = true;
         for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
             const uint32_t r0 = t % g.row_tiles * g.tile_r, v = t / g.row_tiles;
-            for (uint32_t b = 0; b < g.blocks; ++b, ++it) {
-                const uint32_t s = it % kScaleStages;
-                ok = bar_wait(smem_of(&bars.sempty[s]), (it / kScaleStages & 1) ^ 1, lost);
+            for (uint32_t b = 0; b < g.blocks; ++b) {
+                ok = warp_wait(smem_of(&bars.sempty[ring.at]), ring.turn ^ 1, lost);
                 if (!ok) break;
                 const float* src = g.sa + b * g.ld_as + r0;
                 for (uint32_t c = lane; c < g.tile_r; c += 32) {
                     const bool in = r0 + c < g.rows;
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_of(&scales[s][c])),
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_of(&scales[ring.at][c])),
                                  "l"(in ? src + c : g.sa), "r"(in ? 4u : 0u)
                                  : "memory");
                 }
                 if (lane == 0)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_of(&scales[s][kMaxTileR])),
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_of(&scales[ring.at][kNarrowRows])),
                                  "l"(g.sw + v * g.ld_ws + b)
                                  : "memory");
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_of(&bars.sfull[s])) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_of(&bars.sfull[ring.at]))
+                             : "memory");
+                ring.next(kScaleStages);
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp >= 4) {
-        const uint32_t e = warp - 4, quarter = e % 4, half = g.tile_r / 2, c0 = e / 4 * half;
+    } else if (warp >= 4 && warp < 4 + 4 * groups) {
+        const uint32_t e = warp - 4, quarter = e % 4, c0 = e / 4 * 16;
         const uint32_t lanes = tmem + (quarter * 32 << 16) + c0;
-        uint32_t it = 0;
+        Ring ring, buffer;
         bool ok = true;
         for (uint32_t t = blockIdx.x; t < g.tiles; t += gridDim.x) {
-            const uint32_t r0 = t % g.row_tiles * g.tile_r + c0, v = t / g.row_tiles * kTileV + quarter * 32 + lane;
-            float acc[HALF];
+            const uint32_t r0 = t % g.row_tiles * g.tile_r + c0, v = t / g.row_tiles * g.tile_v + quarter * 32 + lane;
+            float acc[16];
 #pragma unroll
-            for (int i = 0; i < HALF; ++i) acc[i] = 0.0f;
-            for (uint32_t b = 0; ok && b < g.blocks; ++b, ++it) {
-                const uint32_t s = it % kScaleStages, buf = it & 1;
-                ok = bar_wait(smem_of(&bars.sfull[s]), it / kScaleStages & 1, lost) &&
-                     bar_wait(smem_of(&bars.tfull[buf]), it / 2 & 1, lost);
-                ok = __all_sync(0xFFFFFFFFu, ok);
+            for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+            for (uint32_t b = 0; ok && b < g.blocks; ++b) {
+                ok = warp_wait(smem_of(&bars.sfull[ring.at]), ring.turn, lost) &&
+                     warp_wait(smem_of(&bars.tfull[buffer.at]), buffer.turn, lost);
                 if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float sw = scales[s][kMaxTileR];
+                tmem_fence_after();
+                float d[16];
+                tmem_load(lanes + buffer.at * g.columns, d);
+                const float sw = scales[ring.at][kNarrowRows];
+                float s[16];
 #pragma unroll
-                for (int c = 0; c < HALF; c += CHUNK) {
-                    if (c < (int)half) {
-                        float d[CHUNK];
-                        tmem_load(lanes + buf * (g.tmem_cols / 2) + c, d);
-                        tmem_wait(d);
-#pragma unroll
-                        for (int i = 0; i < CHUNK; i += 4) {
-                            const float4 sc = *reinterpret_cast<const float4*>(&scales[s][c0 + c + i]);
-                            acc[c + i] = fmaf(d[i], sc.x * sw, acc[c + i]);
-                            acc[c + i + 1] = fmaf(d[i + 1], sc.y * sw, acc[c + i + 1]);
-                            acc[c + i + 2] = fmaf(d[i + 2], sc.z * sw, acc[c + i + 2]);
-                            acc[c + i + 3] = fmaf(d[i + 3], sc.w * sw, acc[c + i + 3]);
-                        }
-                    }
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(&scales[ring.at][c0 + i]);
+                    s[i] = f.x * sw, s[i + 1] = f.y * sw, s[i + 2] = f.z * sw, s[i + 3] = f.w * sw;
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                tmem_wait(d);
+                tmem_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    bar_arrive(smem_of(&bars.tempty[buf]));
-                    bar_arrive(smem_of(&bars.sempty[s]));
+                    bar_arrive(smem_of(&bars.tempty[buffer.at]));
+                    bar_arrive(smem_of(&bars.sempty[ring.at]));
                 }
+                ring.next(kScaleStages);
+                buffer.next(g.buffers);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i] = fmaf(d[i], s[i], acc[i]);
             }
-            // (a wait that ran out leaves NaN, which the samplers report)
             T* out = reinterpret_cast<T*>(g.out) + (uint64_t)r0 * g.ld_out + v;
 #pragma unroll
-            for (int i = 0; i < HALF; ++i)
-                if (i < (int)half && r0 + i < g.rows && v < g.n)
-                    out[i * g.ld_out] = from_float<T>(ok ? acc[i] : __int_as_float(0x7FC00000));
+            for (int i = 0; i < 16; ++i)
+                if (r0 + i < g.rows && v < g.n) out[i * g.ld_out] = from_float<T>(ok ? acc[i] : kLost);
         }
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (warp == 1) {
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
+    tear_down(g, tmem);
+}
+
+// acc += d * s, two columns an instruction
+template <int N>
+__device__ __forceinline__ void add_scaled(float* acc, const float (&d)[N], float s) {
+    const float2 f = make_float2(s, s);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float2 x = __ffma2_rn(make_float2(d[i], d[i + 1]), f, make_float2(acc[i], acc[i + 1]));
+        acc[i] = x.x, acc[i + 1] = x.y;
     }
+}
+
+constexpr uint32_t kWideR = 128, kWideV = 256, kWideWarps = 16;
+constexpr uint32_t kWideCols = kWideV / (kWideWarps / 4);   // of an epilogue warp
+constexpr uint32_t kPiece = 64;                             // bytes of a row that go out together
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                           const __grid_constant__ CUtensorMap map_w, const Args g) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ Barriers bars;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t base = (smem_of(smem) + 1023u) & ~1023u;
+    volatile uint32_t* lost = &bars.lost;
+    const uint32_t tmem = set_up(g, bars, kWideWarps);
+
+    if (warp == 0) {
+        copy_warp(g, bars, base, &map_a, &map_w, false);
+    } else if (warp == 1) {
+        mma_warp(g, bars, base, tmem);
+    } else if (warp >= 4) {
+        const uint32_t e = warp - 4, quarter = e % 4, c0 = e / 4 * kWideCols;
+        const uint32_t lanes = tmem + (quarter * 32 << 16) + c0;
+        uint8_t* piece = smem + (base - smem_of(smem)) + g.stages * g.stage_bytes + e * 32 * kPiece;
+        Ring buffer;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < g.tiles; t += gridDim.x) {
+            const uint32_t r0 = t % g.row_tiles * kWideR + quarter * 32, v0 = t / g.row_tiles * kWideV + c0;
+            // the scales of this thread's row and of its columns' weights, two steps ahead of their use
+            const float* sa = g.sa + min(r0 + lane, g.rows - 1);
+            const float* sw = g.sw + min(v0, g.n - 1) / kBlock * g.ld_ws;
+            float s0 = __ldg(sa) * __ldg(sw), a1 = 0.0f, w1 = 0.0f;
+            if (g.blocks > 1) a1 = __ldg(sa + g.ld_as), w1 = __ldg(sw + 1);
+            float acc[kWideCols];
+#pragma unroll
+            for (int i = 0; i < (int)kWideCols; ++i) acc[i] = 0.0f;
+            for (uint32_t b = 0; ok && b < g.blocks; ++b) {
+                float a2 = 0.0f, w2 = 0.0f;
+                if (b + 2 < g.blocks) a2 = __ldg(sa + (b + 2) * g.ld_as), w2 = __ldg(sw + b + 2);
+                ok = warp_wait(smem_of(&bars.tfull[buffer.at]), buffer.turn, lost);
+                if (!ok) break;
+                tmem_fence_after();
+                const uint32_t from = lanes + buffer.at * g.columns;
+#pragma unroll
+                for (int c = 0; c < (int)kWideCols; c += 16) {
+                    float d[16];
+                    tmem_load(from + c, d);
+                    tmem_wait(d);
+                    add_scaled<16>(acc + c, d, s0);
+                }
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(smem_of(&bars.tempty[buffer.at]));
+                buffer.next(g.buffers);
+                s0 = a1 * w1;
+                a1 = a2, w1 = w2;
+            }
+            // a piece of each of the 32 rows through shared memory: a lane writes its row's 16-byte parts,
+            // turned by the row so that eight rows meet all banks, and lanes read along the rows
+            constexpr uint32_t kCols = kPiece / sizeof(T);
+#pragma unroll
+            for (int c = 0; c < (int)kWideCols; c += kCols) {
+                __syncwarp();
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        if constexpr (sizeof(T) == 4) {
+                            w[i] = __float_as_uint(acc[c + q * 4 + i]);
+                        } else {
+                            const T lo = from_float<T>(acc[c + q * 8 + 2 * i]), hi = from_float<T>(acc[c + q * 8 + 2 * i + 1]);
+                            w[i] = (uint32_t) * reinterpret_cast<const uint16_t*>(&lo) |
+                                   (uint32_t) * reinterpret_cast<const uint16_t*>(&hi) << 16;
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(piece + lane * kPiece + (q ^ (lane >> 1 & 3)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                __syncwarp();
+                constexpr uint32_t kPerRow = kCols, kRows = 32 / kPerRow;
+                const uint32_t col = lane % kPerRow, v = v0 + c + col;
+#pragma unroll 4
+                for (uint32_t i = 0; i < 32; i += kRows) {
+                    const uint32_t row = i + lane / kPerRow, part = col * sizeof(T) / 16;
+                    const T x = *reinterpret_cast<const T*>(piece + row * kPiece + (part ^ (row >> 1 & 3)) * 16 + col * sizeof(T) % 16);
+                    if (r0 + row < g.rows && v < g.n)
+                        reinterpret_cast<T*>(g.out)[(uint64_t)(r0 + row) * g.ld_out + v] = ok ? x : from_float<T>(kLost);
+                }
+            }
+        }
+    }
+    tear_down(g, tmem);
 }
 
 typedef CUresult (*encode_t)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -343,39 +484,52 @@ struct DeviceInfo {
 
 constexpr int kMaxDevices = 64;
 
-template <typename T, int HALF, int CHUNK>
-int launch(const CUtensorMap& mw, const CUtensorMap& ma, Args g, cudaStream_t s) {
+template <typename T>
+int launch(void (*kernel)(CUtensorMap, CUtensorMap, Args), DeviceInfo* info, const CUtensorMap& first,
+           const CUtensorMap& second, Args g, uint32_t more, cudaStream_t s) {
     int dev = 0;
-    static DeviceInfo info[kMaxDevices];  // (every thread that fills an entry writes the same values)
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
         return lrs_call_error(LRS_E_CUDA, "lrs_fp8_logits: no current device");
-    auto* kernel = head_kernel<T, HALF, CHUNK>;
-    if (info[dev].sms == 0) {
+    if (info[dev].sms == 0) {  // (every thread that fills an entry writes the same values)
         int sms = 0, smem = 0;
         cudaFuncAttributes at;
         cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
-        if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kernel);
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, (const void*)kernel);
         if (e == cudaSuccess) smem -= (int)at.sharedSizeBytes;
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return lrs_call_error(LRS_E_CUDA, "lrs_fp8_logits: %s", cudaGetErrorString(e));
         info[dev].smem = smem;
         info[dev].sms = sms;
     }
-    const uint32_t stage = (kTileV + g.tile_r) * kBlock;
-    g.stages = ((uint32_t)info[dev].smem - 1024) / stage;
+    g.stages = ((uint32_t)info[dev].smem - 1024 - more) / g.stage_bytes;
     if (g.stages > kMaxStages) g.stages = kMaxStages;
     const uint32_t grid = g.tiles < (uint32_t)info[dev].sms ? g.tiles : (uint32_t)info[dev].sms;
-    kernel<<<grid, kThreads, g.stages * stage + 1024, s>>>(mw, ma, g);
+    kernel<<<grid, kThreads, g.stages * g.stage_bytes + 1024 + more, s>>>(first, second, g);
     return launched("lrs_fp8_logits");
 }
 
 template <typename T>
-int run(const CUtensorMap& mw, const CUtensorMap& ma, const Args& g, cudaStream_t s) {
-    if (g.tile_r == 16) return launch<T, 8, 8>(mw, ma, g, s);
-    if (g.tile_r <= 64) return launch<T, 32, 16>(mw, ma, g, s);
-    if (g.tile_r <= 128) return launch<T, 64, 16>(mw, ma, g, s);
-    return launch<T, 128, 16>(mw, ma, g, s);
+int run(const uint8_t* d_a, uint64_t ld_a, const uint8_t* d_w, uint64_t ld_w, uint32_t k, Args g, cudaStream_t s) {
+    static DeviceInfo narrow_info[kMaxDevices], wide_info[kMaxDevices];
+    const bool narrow = g.rows <= kNarrowRows;
+    g.tile_r = narrow ? (g.rows + 15) / 16 * 16 : kWideR;
+    g.tile_v = narrow ? 128 : kWideV;
+    g.row_tiles = (g.rows + g.tile_r - 1) / g.tile_r;
+    const uint64_t tiles = (uint64_t)g.row_tiles * ((g.n + g.tile_v - 1) / g.tile_v);
+    if (tiles > 0x7FFFFFFFu) return lrs_call_error(LRS_E_INVALID, "lrs_fp8_logits: rows x n too large");
+    g.tiles = (uint32_t)tiles;
+    g.first_bytes = 128 * kBlock;
+    g.columns = narrow ? g.tile_r : g.tile_v;
+    g.stage_bytes = g.first_bytes + g.columns * kBlock;
+    g.buffers = 512 / g.columns < kMaxBuffers ? 512 / g.columns : kMaxBuffers;
+    g.tmem_columns = 32;
+    while (g.tmem_columns < g.buffers * g.columns) g.tmem_columns *= 2;
+    CUtensorMap ma, mw;
+    if (!code_map(&mw, d_w, g.n, k, ld_w, g.tile_v) || !code_map(&ma, d_a, g.rows, k, ld_a, g.tile_r))
+        return lrs_call_error(LRS_E_INVALID, "lrs_fp8_logits: the codes cannot be mapped (ld too large?)");
+    return narrow ? launch<T>(narrow_kernel<T>, narrow_info, mw, ma, g, 0, s)
+                  : launch<T>(wide_kernel<T>, wide_info, ma, mw, g, kWideWarps * 32 * kPiece, s);
 }
 
 }  // namespace
@@ -401,19 +555,8 @@ extern "C" int lrs_fp8_logits(const uint8_t* d_a, uint64_t ld_a, const float* d_
     g.sa = d_a_scale, g.sw = d_w_scale, g.out = d_out;
     g.ld_as = ld_as, g.ld_ws = ld_ws, g.ld_out = ld_out;
     g.rows = rows, g.n = n, g.blocks = (k + kBlock - 1) / kBlock;
-    // the fewest row tiles of at most 256 rows, of equal size in the tensor core's steps
-    g.row_tiles = (rows + kMaxTileR - 1) / kMaxTileR;
-    const uint32_t each = (rows + g.row_tiles - 1) / g.row_tiles;
-    g.tile_r = each <= 16 ? 16 : (each + 31) / 32 * 32;
-    g.row_tiles = (rows + g.tile_r - 1) / g.tile_r;
-    const uint64_t tiles = (uint64_t)g.row_tiles * ((n + kTileV - 1) / kTileV);
-    if (tiles > 0x7FFFFFFFu) return lrs_call_error(LRS_E_INVALID, "lrs_fp8_logits: rows x n too large");
-    g.tiles = (uint32_t)tiles;
-    g.tmem_cols = 32;
-    while (g.tmem_cols < 2 * g.tile_r) g.tmem_cols *= 2;
-    CUtensorMap mw, ma;
-    if (!code_map(&mw, d_w, n, k, ld_w, kTileV) || !code_map(&ma, d_a, rows, k, ld_a, g.tile_r))
-        return lrs_call_error(LRS_E_INVALID, "lrs_fp8_logits: the codes cannot be mapped (ld too large?)");
     const cudaStream_t s = (cudaStream_t)stream;
-    return out_dtype == LRS_F32 ? run<float>(mw, ma, g, s) : out_dtype == LRS_BF16 ? run<__nv_bfloat16>(mw, ma, g, s) : run<__half>(mw, ma, g, s);
+    return out_dtype == LRS_F32    ? run<float>(d_a, ld_a, d_w, ld_w, k, g, s)
+           : out_dtype == LRS_BF16 ? run<__nv_bfloat16>(d_a, ld_a, d_w, ld_w, k, g, s)
+                                   : run<__half>(d_a, ld_a, d_w, ld_w, k, g, s);
 }
