@@ -3,8 +3,8 @@
 //
 // A block of 128 columns is one step: four tcgen05.mma (kind f8f6f4, K = 32) into TMEM from zero, read
 // back by the epilogue warps and added to f32 registers with the block's scales, while the tensor core
-// fills another TMEM buffer.  Persistent CTAs of twenty warps: 0 issues the TMA copies of both operands
-// (128-byte swizzle, a ring of stages), 1 issues the MMAs, 4-19 are the epilogue.  Tiles walk the row
+// fills another TMEM buffer.  Persistent CTAs: warp 0 issues the TMA copies of both operands
+// (128-byte swizzle, a ring of stages), 1 issues the MMAs, the last 16 are the epilogue.  Tiles walk the row
 // tiles first, so that the CTAs share the weights they stream in L2.  Two forms:
 //   narrow  up to 64 rows (a decode step; bound by the weights' bytes): the weights are the tensor core's
 //           128-row operand, so a few rows cost a narrow instruction and not a padded one, and a warp's
@@ -25,7 +25,7 @@ using namespace lrs;
 
 constexpr uint32_t kBlock = 128;      // columns a scale covers, and columns of a step
 constexpr uint32_t kNarrowRows = 64;  // rows of the narrow form at most
-constexpr uint32_t kThreads = 640;
+constexpr uint32_t kThreads = 640;  // of both forms
 constexpr uint32_t kMaxBuffers = 8;   // TMEM accumulators
 constexpr uint32_t kScaleStages = 8;
 constexpr uint32_t kMaxStages = 10;
@@ -82,10 +82,6 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     *lost = 1;
     return false;
 }
-// The same for a whole warp.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* lost) {
-    return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, lost));
-}
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
     asm volatile(
@@ -123,6 +119,20 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]) :: "memory");
+}
 // Completes the loads: the registers pass through, so that nothing reads them earlier.
 __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -143,6 +153,7 @@ struct Args {
     uint32_t first_bytes, stage_bytes; // of the 128-row operand, of a stage
     uint32_t stages, buffers;          // of shared memory, of TMEM
     uint32_t columns, tmem_columns;    // of a buffer, allocated
+    bool wide_out;                     // rows of d_out start on 16-byte boundaries
 };
 
 struct Barriers {
@@ -195,71 +206,74 @@ __device__ __forceinline__ void tear_down(const Args& g, uint32_t tmem) {
     }
 }
 
-// Warp 0: the copies of both operands of every step; the 128-row operand comes first in a stage.
+// One warp, so that the operands of what its elected lane issues are uniform (as a single thread's they took
+// 800 cycles a step and not 300): the copies of both operands of every step, the 128-row one first.
 __device__ __forceinline__ void copy_warp(const Args& g, Barriers& bars, uint32_t base, const CUtensorMap* first,
-                                          const CUtensorMap* second, bool weights_first) {
+                                            const CUtensorMap* second, bool weights_first) {
     volatile uint32_t* lost = &bars.lost;
+    const uint32_t full = smem_of(bars.full), empty = smem_of(bars.empty);
+    const bool leader = elect();
     Ring ring;
-    uint32_t issued = 0;
+    uint32_t at = base, issued = 0;
     bool ok = true;
     for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
         const uint32_t r0 = t % g.row_tiles * g.tile_r, v0 = t / g.row_tiles * g.tile_v;
         const uint32_t y0 = weights_first ? v0 : r0, y1 = weights_first ? r0 : v0;
-        for (uint32_t b = 0; b < g.blocks; ++b) {
-            ok = warp_wait(smem_of(&bars.empty[ring.at]), ring.turn ^ 1, lost);
+        for (uint32_t b = 0; b < g.blocks; ++b, ++issued) {
+            ok = bar_wait(empty + ring.at * 8, ring.turn ^ 1, lost);
             if (!ok) break;
-            if (elect()) {
-                const uint32_t bar = smem_of(&bars.full[ring.at]), at = base + ring.at * g.stage_bytes;
+            const uint32_t bar = full + ring.at * 8;
+            if (leader) {
                 bar_expect(bar, g.stage_bytes);
                 tma_load(at, first, b * kBlock, y0, bar);
                 tma_load(at + g.first_bytes, second, b * kBlock, y1, bar);
             }
-            __syncwarp();
             ring.next(g.stages);
-            ++issued;
+            at = ring.at == 0 ? base : at + g.stage_bytes;
         }
     }
     if (!ok) {  // copies that a warp which gave up did not wait for land before the CTA ends
         for (uint32_t j = issued > g.stages ? issued - g.stages : 0; j < issued; ++j) {
             const long long t0 = clock64();
-            while (!bar_try(smem_of(&bars.full[j % g.stages]), j / g.stages & 1) && clock64() - t0 < kWaitCycles) {
+            while (!bar_try(full + j % g.stages * 8, j / g.stages & 1) && clock64() - t0 < kWaitCycles) {
             }
         }
     }
 }
 
-// Warp 1: the MMAs of every step, 128 x `columns` into the next TMEM buffer.
+// One warp: the MMAs of every step, 128 x `columns` into the next TMEM buffer.
 __device__ __forceinline__ void mma_warp(const Args& g, Barriers& bars, uint32_t base, uint32_t tmem) {
     volatile uint32_t* lost = &bars.lost;
     const uint32_t idesc = 1u << 4 | g.columns / 8 << 17 | 128 / 16 << 24;  // f32 += e4m3 x e4m3, both K-major
+    const uint32_t full = smem_of(bars.full), empty = smem_of(bars.empty), tfull = smem_of(bars.tfull), tempty = smem_of(bars.tempty);
+    const uint64_t first = operand(base), second = operand(base + g.first_bytes), step = g.stage_bytes >> 4;
+    const bool leader = elect();
     Ring ring, buffer;
+    uint64_t da = first, db = second;
+    uint32_t d = tmem;
     bool ok = true;
     for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
         for (uint32_t b = 0; b < g.blocks; ++b) {
-            ok = warp_wait(smem_of(&bars.tempty[buffer.at]), buffer.turn ^ 1, lost) &&
-                 warp_wait(smem_of(&bars.full[ring.at]), ring.turn, lost);
+            ok = bar_wait(tempty + buffer.at * 8, buffer.turn ^ 1, lost) && bar_wait(full + ring.at * 8, ring.turn, lost);
             if (!ok) break;
             tmem_fence_after();
-            if (elect()) {
-                const uint32_t at = base + ring.at * g.stage_bytes, d = tmem + buffer.at * g.columns;
-                const uint64_t da = operand(at), db = operand(at + g.first_bytes);
+            if (leader) {
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) mma(d, da + 2 * j, db + 2 * j, idesc, j > 0);
-                mma_commit(smem_of(&bars.empty[ring.at]));
-                mma_commit(smem_of(&bars.tfull[buffer.at]));
+                mma_commit(empty + ring.at * 8);
+                mma_commit(tfull + buffer.at * 8);
             }
-            __syncwarp();
             ring.next(g.stages);
             buffer.next(g.buffers);
+            da = ring.at == 0 ? first : da + step, db = ring.at == 0 ? second : db + step;
+            d = buffer.at == 0 ? tmem : d + g.columns;
         }
     }
     // every MMA has ended before the TMEM goes back
-    if (elect()) mma_commit(smem_of(&bars.drain));
-    __syncwarp();
+    if (leader) mma_commit(smem_of(&bars.drain));
     const long long t0 = clock64();
     while (!bar_try(smem_of(&bars.drain), 0) && clock64() - t0 < kWaitCycles) {
     }
-    __syncwarp();
 }
 
 constexpr float kLost = __builtin_nanf("");  // what a wait that ran out leaves: the samplers report it
@@ -285,8 +299,8 @@ __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_consta
         for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
             const uint32_t r0 = t % g.row_tiles * g.tile_r, v = t / g.row_tiles;
             for (uint32_t b = 0; b < g.blocks; ++b) {
-                ok = warp_wait(smem_of(&bars.sempty[ring.at]), ring.turn ^ 1, lost);
-                if (!ok) break;
+                ok = bar_wait(smem_of(&bars.sempty[ring.at]), ring.turn ^ 1, lost);
+                if (!ok) break;  // (a lane that gives up sends nothing more: the others run out as well)
                 const float* src = g.sa + b * g.ld_as + r0;
                 for (uint32_t c = lane; c < g.tile_r; c += 32) {
                     const bool in = r0 + c < g.rows;
@@ -314,10 +328,11 @@ __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_consta
             float acc[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-            for (uint32_t b = 0; ok && b < g.blocks; ++b) {
-                ok = warp_wait(smem_of(&bars.sfull[ring.at]), ring.turn, lost) &&
-                     warp_wait(smem_of(&bars.tfull[buffer.at]), buffer.turn, lost);
-                if (!ok) break;
+            // (after a wait that ran out the steps go on without waiting, and the tile is lost)
+            for (uint32_t b = 0; b < g.blocks; ++b) {
+                ok &= bar_wait(smem_of(&bars.sfull[ring.at]), ring.turn, lost);
+                ok &= bar_wait(smem_of(&bars.tfull[buffer.at]), buffer.turn, lost);
+                __syncwarp();
                 tmem_fence_after();
                 float d[16];
                 tmem_load(lanes + buffer.at * g.columns, d);
@@ -362,6 +377,8 @@ __device__ __forceinline__ void add_scaled(float* acc, const float (&d)[N], floa
 
 constexpr uint32_t kWideR = 128, kWideV = 256, kWideWarps = 16;
 constexpr uint32_t kWideCols = kWideV / (kWideWarps / 4);   // of an epilogue warp
+constexpr uint32_t kFewRegs = 32, kManyRegs = 112;          // of the first four warps, of the epilogue's
+constexpr uint32_t kWideRegs = 128 * kFewRegs + 512 * kManyRegs;
 constexpr uint32_t kPiece = 64;                             // bytes of a row that go out together
 
 template <typename T>
@@ -373,51 +390,59 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     const uint32_t base = (smem_of(smem) + 1023u) & ~1023u;
     volatile uint32_t* lost = &bars.lost;
     const uint32_t tmem = set_up(g, bars, kWideWarps);
-
-    if (warp == 0) {
-        copy_warp(g, bars, base, &map_a, &map_w, false);
-    } else if (warp == 1) {
-        mma_warp(g, bars, base, tmem);
-    } else if (warp >= 4) {
-        const uint32_t e = warp - 4, quarter = e % 4, c0 = e / 4 * kWideCols;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+        if (warp == 0) copy_warp(g, bars, base, &map_a, &map_w, false);
+        if (warp == 1) mma_warp(g, bars, base, tmem);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
+        const uint32_t e = warp - 4, quarter = warp % 4, c0 = e / 4 * kWideCols;
         const uint32_t lanes = tmem + (quarter * 32 << 16) + c0;
+        const uint32_t tfull = smem_of(bars.tfull), tempty = smem_of(bars.tempty);
         uint8_t* piece = smem + (base - smem_of(smem)) + g.stages * g.stage_bytes + e * 32 * kPiece;
-        Ring buffer;
+        uint32_t buffer = 0, turn = 0;
         bool ok = true;
         for (uint32_t t = blockIdx.x; t < g.tiles; t += gridDim.x) {
             const uint32_t r0 = t % g.row_tiles * kWideR + quarter * 32, v0 = t / g.row_tiles * kWideV + c0;
-            // the scales of this thread's row and of its columns' weights, two steps ahead of their use
+            // the scales of this thread's row and of its columns' weights, a step ahead of their use
             const float* sa = g.sa + min(r0 + lane, g.rows - 1);
             const float* sw = g.sw + min(v0, g.n - 1) / kBlock * g.ld_ws;
-            float s0 = __ldg(sa) * __ldg(sw), a1 = 0.0f, w1 = 0.0f;
-            if (g.blocks > 1) a1 = __ldg(sa + g.ld_as), w1 = __ldg(sw + 1);
+            float a1 = __ldg(sa), w1 = __ldg(sw);
             float acc[kWideCols];
 #pragma unroll
             for (int i = 0; i < (int)kWideCols; ++i) acc[i] = 0.0f;
-            for (uint32_t b = 0; ok && b < g.blocks; ++b) {
-                float a2 = 0.0f, w2 = 0.0f;
-                if (b + 2 < g.blocks) a2 = __ldg(sa + (b + 2) * g.ld_as), w2 = __ldg(sw + b + 2);
-                ok = warp_wait(smem_of(&bars.tfull[buffer.at]), buffer.turn, lost);
-                if (!ok) break;
+            // (after a wait that ran out the steps go on without waiting, and the tile is lost)
+            for (uint32_t b = 0; b < g.blocks; ++b) {
+                const float s0 = a1 * w1;
+                if (b + 1 < g.blocks) sa += g.ld_as, ++sw, a1 = __ldg(sa), w1 = __ldg(sw);
+                ok &= bar_wait(tfull + buffer * 8, turn, lost);
+                __syncwarp();
                 tmem_fence_after();
-                const uint32_t from = lanes + buffer.at * g.columns;
+                const uint32_t from = lanes + buffer * kWideV;
 #pragma unroll
-                for (int c = 0; c < (int)kWideCols; c += 16) {
-                    float d[16];
+                for (int c = 0; c < (int)kWideCols; c += 32) {
+                    float d[32];
                     tmem_load(from + c, d);
                     tmem_wait(d);
-                    add_scaled<16>(acc + c, d, s0);
+                    if (c + 32 == (int)kWideCols) {
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(tempty + buffer * 8);
+                    }
+                    add_scaled<32>(acc + c, d, s0);
                 }
-                tmem_fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(smem_of(&bars.tempty[buffer.at]));
-                buffer.next(g.buffers);
-                s0 = a1 * w1;
-                a1 = a2, w1 = w2;
+                buffer ^= 1;
+                turn ^= buffer == 0;
+            }
+            if (!ok) {
+#pragma unroll
+                for (int i = 0; i < (int)kWideCols; ++i) acc[i] = kLost;
             }
             // a piece of each of the 32 rows through shared memory: a lane writes its row's 16-byte parts,
             // turned by the row so that eight rows meet all banks, and lanes read along the rows
-            constexpr uint32_t kCols = kPiece / sizeof(T);
+            constexpr uint32_t kCols = kPiece / sizeof(T), kEach = 16 / sizeof(T);
+            T* out = reinterpret_cast<T*>(g.out) + (uint64_t)r0 * g.ld_out + v0;
+            const uint32_t left = r0 < g.rows ? g.rows - r0 : 0;  // rows of this warp's 32
 #pragma unroll
             for (int c = 0; c < (int)kWideCols; c += kCols) {
                 __syncwarp();
@@ -437,14 +462,24 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
                     *reinterpret_cast<uint4*>(piece + lane * kPiece + (q ^ (lane >> 1 & 3)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
                 __syncwarp();
-                constexpr uint32_t kPerRow = kCols, kRows = 32 / kPerRow;
-                const uint32_t col = lane % kPerRow, v = v0 + c + col;
-#pragma unroll 4
-                for (uint32_t i = 0; i < 32; i += kRows) {
-                    const uint32_t row = i + lane / kPerRow, part = col * sizeof(T) / 16;
-                    const T x = *reinterpret_cast<const T*>(piece + row * kPiece + (part ^ (row >> 1 & 3)) * 16 + col * sizeof(T) % 16);
-                    if (r0 + row < g.rows && v < g.n)
-                        reinterpret_cast<T*>(g.out)[(uint64_t)(r0 + row) * g.ld_out + v] = ok ? x : from_float<T>(kLost);
+                if (g.wide_out && v0 + c + kCols <= g.n) {  // 16 bytes a lane, eight rows an instruction
+                    const uint32_t row0 = lane / 4, part = lane % 4;
+                    T* to = out + row0 * g.ld_out + c + part * kEach;
+#pragma unroll
+                    for (uint32_t row = row0; row < 32; row += 8, to += 8 * g.ld_out) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(piece + row * kPiece + (part ^ (row >> 1 & 3)) * 16);
+                        if (row < left) *reinterpret_cast<uint4*>(to) = x;
+                    }
+                } else {
+                    constexpr uint32_t kRows = 32 / kCols;  // rows an instruction
+                    const uint32_t row0 = lane / kCols, col = lane % kCols, part = col / kEach;
+                    const uint32_t end = v0 + c + col < g.n ? left : 0;
+                    T* to = out + row0 * g.ld_out + c + col;
+#pragma unroll 8
+                    for (uint32_t row = row0; row < 32; row += kRows, to += kRows * g.ld_out) {
+                        const T x = *reinterpret_cast<const T*>(piece + row * kPiece + (part ^ (row >> 1 & 3)) * 16 + col * sizeof(T) % 16);
+                        if (row < end) *to = x;
+                    }
                 }
             }
         }
@@ -486,7 +521,7 @@ constexpr int kMaxDevices = 64;
 
 template <typename T>
 int launch(void (*kernel)(CUtensorMap, CUtensorMap, Args), DeviceInfo* info, const CUtensorMap& first,
-           const CUtensorMap& second, Args g, uint32_t more, cudaStream_t s) {
+           const CUtensorMap& second, Args g, uint32_t regs, uint32_t more, cudaStream_t s) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
         return lrs_call_error(LRS_E_CUDA, "lrs_fp8_logits: no current device");
@@ -496,6 +531,10 @@ int launch(void (*kernel)(CUtensorMap, CUtensorMap, Args), DeviceInfo* info, con
         cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
         if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, (const void*)kernel);
+        // the registers that the warps' shares add up to are there from the launch on: a share would be
+        // waited for in vain otherwise
+        if (e == cudaSuccess && (uint32_t)at.numRegs * kThreads < regs)
+            return lrs_call_error(LRS_E_INTERNAL, "lrs_fp8_logits: %d registers a thread at launch", at.numRegs);
         if (e == cudaSuccess) smem -= (int)at.sharedSizeBytes;
         if (e == cudaSuccess) e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return lrs_call_error(LRS_E_CUDA, "lrs_fp8_logits: %s", cudaGetErrorString(e));
@@ -525,11 +564,12 @@ int run(const uint8_t* d_a, uint64_t ld_a, const uint8_t* d_w, uint64_t ld_w, ui
     g.buffers = 512 / g.columns < kMaxBuffers ? 512 / g.columns : kMaxBuffers;
     g.tmem_columns = 32;
     while (g.tmem_columns < g.buffers * g.columns) g.tmem_columns *= 2;
+    g.wide_out = (uintptr_t)g.out % 16 == 0 && (g.rows == 1 || g.ld_out * sizeof(T) % 16 == 0);
     CUtensorMap ma, mw;
     if (!code_map(&mw, d_w, g.n, k, ld_w, g.tile_v) || !code_map(&ma, d_a, g.rows, k, ld_a, g.tile_r))
         return lrs_call_error(LRS_E_INVALID, "lrs_fp8_logits: the codes cannot be mapped (ld too large?)");
-    return narrow ? launch<T>(narrow_kernel<T>, narrow_info, mw, ma, g, 0, s)
-                  : launch<T>(wide_kernel<T>, wide_info, ma, mw, g, kWideWarps * 32 * kPiece, s);
+    return narrow ? launch<T>(narrow_kernel<T>, narrow_info, mw, ma, g, 0, 0, s)
+                  : launch<T>(wide_kernel<T>, wide_info, ma, mw, g, kWideRegs, kWideWarps * 32 * kPiece, s);
 }
 
 }  // namespace
