@@ -7,9 +7,9 @@
 //
 // A row is one cluster of CTAs (one CTA for batches, up to 16 for a few rows), each with a slice of
 // its tiles of 1024 elements; nothing is kept outside shared memory.
-//   1. One pass over the logits: the maximum of every 16-byte-by-32-lane chunk and, where the whole
-//      row's mass Z is asked for, the tile's sum of weights, all written to the first CTA (over
-//      distributed shared memory).  With filters the sums are 32-bit ones, good to kApprox = 2^-20.
+//   1. One pass over the logits: the maximum of every chunk of 128 elements and, where the whole row's
+//      mass Z is asked for, the tile's sum of weights, all written to the first CTA (over distributed
+//      shared memory).  With filters the sums are 32-bit ones, good to kApprox = 2^-20.
 //   2. Few survivors (the first CTA): the k-th largest chunk maximum is a lower bound of the k-th
 //      largest logit; maxima whose mass reaches top_p Z bound the nucleus; min-p bounds directly.
 //      The chunks that reach the bound are read again, what reaches it goes to a list, the list is
@@ -30,11 +30,14 @@ namespace {
 using namespace lrs;
 namespace cg = cooperative_groups;
 
-constexpr uint32_t kThreads = 512;
+constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWarps = kThreads / 32;
 constexpr uint32_t kTile = 1024;       // elements of a tile, 32 a lane
-constexpr uint32_t kList = 4096;       // candidates that are sorted
+constexpr uint32_t kList = 4096;       // candidates that are listed
+constexpr uint32_t kChunk = 128;       // elements of a chunk
+constexpr uint32_t kPer = kTile / kChunk;
 constexpr uint32_t kChunks = 2048;     // chunks that are read again for them
+constexpr uint32_t kFew = kThreads;    // candidates that are ranked without a sort
 constexpr uint32_t kBins = 4096;
 constexpr uint32_t kMaxCluster = 16;
 constexpr uint32_t kAll = 0xFFFFFFFFu;
@@ -85,19 +88,39 @@ struct Sum {
 // Units of a weight of 1 in a bin's mass: the sum of n of them stays below 2^31.
 __device__ __forceinline__ uint32_t mass_unit(uint32_t n) { return 1u << (__clz((n - 1) | 1) - 2); }
 
+// A candidate's test: above the bound that the chunk maxima gave.  The distance from the maximum, in 256ths
+// of the maxima's range and in a second round in 256ths of one of those, is a monotone function of x, so
+// that a bound on it is one on x.
+struct Bound {
+    float top, scale, least;  // nothing below `least` is kept
+    float edge0, edge1;       // candidates: distance < edge0 - 1, or within one below edge0 and the rest < edge1
+    bool bounded;
+    __device__ __forceinline__ float distance(float x) const { return (0.5f * top - 0.5f * x) * scale; }
+    __device__ __forceinline__ bool operator()(float x) const {
+        const float f = distance(x);
+        return x >= least && (!bounded || f < edge0 - 1.0f || (f < edge0 && (f - (edge0 - 1.0f)) * 256.0f < edge1));
+    }
+};
+
 struct Shared {
     Sum part[kWarps];
     Sum from[kMaxCluster];       // (first CTA: the others' sums)
     float top[kWarps], tops[kMaxCluster];
     uint32_t word[kWarps];
+    uint64_t wide[kWarps];
     uint32_t order[4];           // what the first CTA has all do next: operation, upper and lower key, shift
+    Bound bound;
     uint32_t count, chunks;      // entries of the lists
     uint64_t cut;
 };
 
-enum { kDone, kHistogram, kSumAbove, kGather, kGatherTies };
+enum { kDone, kHistogram, kSumAbove, kGather, kGatherTies, kCandidates };
 
 __device__ __forceinline__ Sum add(const Sum& a, const Sum& b) { return Sum{a.n + b.n, a.lo + b.lo, a.hi + b.hi}; }
+
+__device__ __forceinline__ Sum shift_up(const Sum& v, int o) {
+    return Sum{__shfl_up_sync(kAll, v.n, o), __shfl_up_sync(kAll, v.lo, o), __shfl_up_sync(kAll, v.hi, o)};
+}
 
 // Sums over the CTA in one order; every thread gets the total, and the sum of the threads before it.
 __device__ __noinline__ Sum block_scan(Sum v, Sum* before, Shared& sh) {
@@ -105,22 +128,28 @@ __device__ __noinline__ Sum block_scan(Sum v, Sum* before, Shared& sh) {
     Sum inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-        Sum p{__shfl_up_sync(kAll, inc.n, o), __shfl_up_sync(kAll, inc.lo, o), __shfl_up_sync(kAll, inc.hi, o)};
+        const Sum p = shift_up(inc, o);
         if (lane >= o) inc = add(p, inc);
     }
     __syncthreads();
     if (lane == 31) sh.part[warp] = inc;
     __syncthreads();
-    Sum t{0, 0.0, 0.0}, w{0, 0.0, 0.0};
-    for (uint32_t i = 0; i < kWarps; ++i) {
-        if (i == warp) w = t;
-        t = add(t, sh.part[i]);
+    Sum w = lane < kWarps ? sh.part[lane] : Sum{0, 0.0, 0.0};
+#pragma unroll
+    for (int o = 1; o < (int)kWarps; o *= 2) {
+        const Sum p = shift_up(w, o);
+        if (lane >= o) w = add(p, w);
     }
     if (before) {
-        Sum p{__shfl_up_sync(kAll, inc.n, 1), __shfl_up_sync(kAll, inc.lo, 1), __shfl_up_sync(kAll, inc.hi, 1)};
-        *before = lane ? add(w, p) : w;
+        const Sum in_warp = shift_up(inc, 1);
+        const uint32_t last = warp ? warp - 1 : 0;
+        const Sum warps{__shfl_sync(kAll, w.n, last), __shfl_sync(kAll, w.lo, last), __shfl_sync(kAll, w.hi, last)};
+        Sum r{0, 0.0, 0.0};
+        if (warp) r = warps;
+        if (lane) r = add(r, in_warp);
+        *before = r;
     }
-    return t;
+    return Sum{__shfl_sync(kAll, w.n, kWarps - 1), __shfl_sync(kAll, w.lo, kWarps - 1), __shfl_sync(kAll, w.hi, kWarps - 1)};
 }
 
 __device__ __noinline__ uint32_t block_min(uint32_t v, Shared& sh) {
@@ -128,30 +157,123 @@ __device__ __noinline__ uint32_t block_min(uint32_t v, Shared& sh) {
     __syncthreads();
     if (threadIdx.x % 32 == 0) sh.word[threadIdx.x / 32] = v;
     __syncthreads();
-    for (uint32_t i = 0; i < kWarps; ++i) v = min(v, sh.word[i]);
-    return v;
+    return __reduce_min_sync(kAll, sh.word[threadIdx.x % kWarps]);
 }
 
-// Bitonic sort of list[0 .. 2^m) (2^m >= count, entries from count on given `pad` here), ascending or
-// descending.  Steps whose pairs stay within a warp's 64 entries need no barrier of the CTA.
-template <bool DESC>
+__device__ __noinline__ float block_min_float(float v, Shared& sh) {
+    const uint32_t key = block_min(key_of(v), sh);
+    return value_of(key);
+}
+
+// Sums of two words over the threads before each.
+__device__ __noinline__ void block_scan_words(uint32_t a, uint32_t b, uint32_t* before_a, uint32_t* before_b, Shared& sh) {
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    uint32_t ia = a, ib = b;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t qa = __shfl_up_sync(kAll, ia, o), qb = __shfl_up_sync(kAll, ib, o);
+        if (lane >= o) ia += qa, ib += qb;
+    }
+    __syncthreads();
+    if (lane == 31) sh.part[warp].n = ia, sh.word[warp] = ib;
+    __syncthreads();
+    const uint32_t wa = __reduce_add_sync(kAll, lane < warp ? sh.part[lane].n : 0), wb = __reduce_add_sync(kAll, lane < warp ? sh.word[lane] : 0);
+    *before_a = wa + ia - a, *before_b = wb + ib - b;
+}
+
+// Sum over the threads before each, and of all.
+__device__ __noinline__ uint64_t block_scan_long(uint64_t v, uint64_t* before, Shared& sh) {
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    uint64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint64_t q = __shfl_up_sync(kAll, inc, o);
+        if (lane >= o) inc += q;
+    }
+    __syncthreads();
+    if (lane == 31) sh.wide[warp] = inc;
+    __syncthreads();
+    uint64_t first = 0, all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kWarps; ++i) {
+        if (i == warp) first = all;
+        all += sh.wide[i];
+    }
+    *before = first + inc - v;
+    return all;
+}
+
+// Bitonic sort of list[0 .. 2^m) (2^m >= count, zeros from count on written here), descending.  Steps
+// whose pairs stay within a warp's 64 entries need no barrier of the CTA.
 __device__ __noinline__ void sort(uint64_t* list, uint32_t count) {
     uint32_t size = 2;
     while (size < count) size *= 2;
-    for (uint32_t i = count + threadIdx.x; i < size; i += kThreads) list[i] = DESC ? 0ull : ~0ull;
+    for (uint32_t i = count + threadIdx.x; i < size; i += kThreads) list[i] = 0;
     __syncthreads();
     for (uint32_t m = 2; m <= size; m *= 2)
         for (uint32_t j = m / 2; j > 0; j /= 2) {
             for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
                 const uint32_t i = 2 * t - (t & (j - 1));
                 const uint64_t a = list[i], b = list[i + j];
-                if ((a > b) != (((i & m) != 0) ^ DESC)) list[i] = b, list[i + j] = a;
+                if ((a < b) == ((i & m) == 0)) list[i] = b, list[i + j] = a;
             }
             if (j > 32 || (j == 1 && m >= 64) || size / 2 > kThreads)
                 __syncthreads();
             else
                 __syncwarp();
         }
+    __syncthreads();
+}
+
+constexpr uint32_t kSlots = 512;  // of the bins below
+constexpr uint32_t kOwn = kList / kThreads;
+
+// order[i] = place in the list of its i-th largest entry: entries are dealt into bins by their value
+// between the list's ends, and ranked within their bin by comparison.  Lists that crowd a bin (long runs
+// of equal values) are sorted in place.
+__device__ __noinline__ void rank_list(uint64_t* list, uint16_t* order, uint32_t* slots, uint32_t count, Shared& sh) {
+    uint32_t* ends = slots + kSlots;
+    uint32_t least = kAll, most = 0;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t key = (uint32_t)(list[i] >> 32);
+        least = min(least, key), most = max(most, key);
+    }
+    const float low = value_of(block_min(least, sh)), top = value_of(~block_min(~most, sh));
+    const float scale = low < top ? fminf((float)kSlots * 0.999f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f;
+    auto slot = [&](uint64_t entry) {
+        return min((uint32_t)((0.5f * top - 0.5f * value_of((uint32_t)(entry >> 32))) * scale), kSlots - 1);
+    };
+    for (uint32_t i = threadIdx.x; i < kSlots; i += kThreads) slots[i] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) atomicAdd(&slots[slot(list[i])], 1u);
+    __syncthreads();
+    const uint32_t a = slots[2 * threadIdx.x], b = slots[2 * threadIdx.x + 1];
+    uint32_t before, unused;
+    block_scan_words(a + b, 0, &before, &unused, sh);
+    ends[2 * threadIdx.x] = before, ends[2 * threadIdx.x + 1] = before + a;
+    if (__syncthreads_or(a > kSlots || b > kSlots)) {
+        sort(list, count);
+        for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[i] = (uint16_t)i;
+        __syncthreads();
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[atomicAdd(&ends[slot(list[i])], 1u)] = (uint16_t)i;
+    __syncthreads();
+    uint16_t place[kOwn];
+#pragma unroll
+    for (uint32_t q = 0; q < kOwn; ++q) {
+        const uint32_t i = threadIdx.x + q * kThreads;
+        if (i >= count) break;
+        const uint64_t entry = list[i];
+        const uint32_t s = slot(entry), end = ends[s];
+        uint32_t rank = end - slots[s];
+        for (uint32_t j = rank; j < end; ++j) rank += list[order[j]] > entry;
+        place[q] = (uint16_t)rank;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t q = 0; q < kOwn; ++q)
+        if (threadIdx.x + q * kThreads < count) order[place[q]] = (uint16_t)(threadIdx.x + q * kThreads);
     __syncthreads();
 }
 
@@ -170,7 +292,7 @@ struct Args {
 // The row as this call sees it: element i at base[i + skew], base on a 16-byte boundary.
 template <typename T>
 struct RowView {
-    static constexpr uint32_t kVec = 16 / sizeof(T), kChunk = 32 * kVec, kPer = kTile / kChunk;
+    static constexpr uint32_t kVec = 16 / sizeof(T), kLoad = 32 * kVec, kLoads = kTile / kLoad;  // of a warp
     const T* base;
     uint32_t skew, end;  // elements are base[skew .. end)
 
@@ -186,14 +308,31 @@ struct RowView {
             for (uint32_t i = 0; i < kVec; ++i) v[i] = j + i >= skew && j + i < end ? to_float<T>(base[j + i]) : -INFINITY;
         }
     }
+    // four elements from position j (a multiple of four)
+    __device__ __forceinline__ void quad(uint32_t j, float (&v)[4]) const {
+        if (j >= skew && j + 4 <= end) {
+            if constexpr (sizeof(T) == 4) {
+                unpack(__ldg(reinterpret_cast<const uint4*>(base + j)), v, base);
+            } else {
+                const uint2 q = __ldg(reinterpret_cast<const uint2*>(base + j));
+                float x[8];
+                unpack(make_uint4(q.x, q.y, 0, 0), x, base);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = x[i];
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) v[i] = j + i >= skew && j + i < end ? to_float<T>(base[j + i]) : -INFINITY;
+        }
+    }
     __device__ __forceinline__ void tile(uint32_t t, float (&v)[32]) const {
         const uint32_t j = t * kTile + threadIdx.x % 32 * kVec;
         if (t * kTile >= skew && t * kTile + kTile <= end) {
-            uint4 r[kPer];
+            uint4 r[kLoads];
 #pragma unroll
-            for (uint32_t c = 0; c < kPer; ++c) r[c] = __ldg(reinterpret_cast<const uint4*>(base + j + c * kChunk));
+            for (uint32_t c = 0; c < kLoads; ++c) r[c] = __ldg(reinterpret_cast<const uint4*>(base + j + c * kLoad));
 #pragma unroll
-            for (uint32_t c = 0; c < kPer; ++c) {
+            for (uint32_t c = 0; c < kLoads; ++c) {
                 float x[kVec];
                 unpack(r[c], x, base);
 #pragma unroll
@@ -201,8 +340,28 @@ struct RowView {
             }
         } else {
 #pragma unroll
-            for (uint32_t c = 0; c < kPer; ++c) vec(j + c * kChunk, v + c * kVec);
+            for (uint32_t c = 0; c < kLoads; ++c) vec(j + c * kLoad, v + c * kVec);
         }
+    }
+    // the maxima of the tile's chunks: lane i < kPer gets chunk i's; a NaN stays
+    __device__ __forceinline__ float chunk_max(const float (&v)[32], float* all) const {
+        const uint32_t lane = threadIdx.x % 32;
+        float mine = 0.0f, top = -INFINITY;
+#pragma unroll
+        for (uint32_t c = 0; c < kLoads; ++c) {
+            float m = v[c * kVec];
+#pragma unroll
+            for (uint32_t e = 1; e < kVec; ++e) m = max_nan(m, v[c * kVec + e]);
+            constexpr uint32_t kIn = kLoad / kChunk;  // chunks of a load: 1, or one a half-warp
+#pragma unroll
+            for (uint32_t h = 0; h < kIn; ++h) {
+                const float w = warp_max_nan(kIn == 1 || lane / 16 == h ? m : -INFINITY);
+                if (lane == c * kIn + h) mine = w;
+                top = max_nan(top, w);
+            }
+        }
+        *all = top;
+        return mine;
     }
 };
 
@@ -247,6 +406,30 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
+// Appends the elements of a lane's bit mask to the first CTA's list: one addition to its count a warp.
+template <typename T, int N, typename Index>
+__device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const float (&v)[N], uint32_t mask, Index index) {
+    const uint32_t lane = threadIdx.x % 32, mine = __popc(mask);
+    uint32_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t q = __shfl_up_sync(kAll, inc, o);
+        if (lane >= o) inc += q;
+    }
+    const uint32_t all = __shfl_sync(kAll, inc, 31);
+    if (all == 0) return;
+    uint32_t at = 0;
+    if (lane == 31) at = atomicAdd(count, all);
+    at = __shfl_sync(kAll, at, 31) + inc - mine;
+    if (mask == 0) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (!(mask >> i & 1)) continue;
+        if (at < kList) list[at] = (uint64_t)key_of(v[i]) << 32 | ~index(i);
+        ++at;
+    }
+}
+
 // One operation of the first CTA's over this CTA's slice of the row: keys from `hi` up are summed, those
 // of [lo, hi) counted by bin, listed, or counted by tile.
 template <typename T>
@@ -272,7 +455,9 @@ __device__ __noinline__ void perform(const Slice<T>& z, float max, Shared& sh) {
     const Weigh weigh{(double)max, z.c};
     const float cf = (float)z.c, scale = (float)mass_unit(z.n);
     Sum s{0, 0.0, 0.0};  // elements from hi up: count and mass; mass of all (histograms)
-    if (op == kHistogram) {
+    const Bound bound = sh.bound;
+    const uint32_t rank = cluster.block_rank();
+    if (op == kHistogram && rank) {  // (the first CTA's bins are clear: the others' come to them)
         for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads) bin_n[i] = 0;
         __syncthreads();
     }
@@ -299,46 +484,39 @@ __device__ __noinline__ void perform(const Slice<T>& z, float max, Shared& sh) {
             }
             continue;
         }
-        uint32_t ties = 0;
+        auto index = [&](int i) { return t * kTile + i / View::kVec * View::kLoad + lane * View::kVec + i % View::kVec - z.row.skew; };
+        uint32_t mask = 0;
+        if (op == kCandidates) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mask |= bound(v[i]) ? 1u << i : 0u;
+            append<T>(first_list, first_count, v, mask, index);
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const uint32_t key = key_of(v[i]);
             if (key >= hi) above += weigh(v[i]), ++s.n;
-            ties += key >= lo && key < hi;
+            mask |= key >= lo && key < hi ? 1u << i : 0u;
         }
         s.lo += above;
         if (op == kSumAbove) continue;
         above = warp_sum(above);
         if (lane == 0) z.first_sum[t] = above;
         if (op == kGatherTies) {
-            ties = __reduce_add_sync(kAll, ties);
+            const uint32_t ties = __reduce_add_sync(kAll, __popc(mask));
             if (lane == 0) reinterpret_cast<uint32_t*>(z.first_max)[t] = ties;
         } else {
-            // the lane's place in the list, then its elements in turn
-            uint32_t inc = ties;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const uint32_t q = __shfl_up_sync(kAll, inc, o);
-                if (lane >= o) inc += q;
-            }
-            const uint32_t all = __shfl_sync(kAll, inc, 31);
-            if (all == 0) continue;
-            uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(first_count, all);
-            at = __shfl_sync(kAll, at, 0) + inc - ties;
-            if (ties == 0) continue;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const uint32_t key = key_of(v[i]);
-                if (key < lo || key >= hi) continue;
-                const uint32_t index = t * kTile + i / View::kVec * View::kChunk + lane * View::kVec + i % View::kVec - z.row.skew;
-                if (at < kList) first_list[at] = (uint64_t)key << 32 | ~index;
-                ++at;
-            }
+            append<T>(first_list, first_count, v, mask, index);
         }
     }
+    if (op == kHistogram && rank) {
+        __syncthreads();
+        uint32_t* first_bin = cluster.map_shared_rank(bin_n, 0);
+        for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads)
+            if (bin_n[i]) atomicAdd(&first_bin[i], bin_n[i]);
+    }
     s = block_scan(s, nullptr, sh);
-    if (threadIdx.x == 0) *cluster.map_shared_rank(&sh.from[cluster.block_rank()], 0) = s;
+    if (threadIdx.x == 0) *cluster.map_shared_rank(&sh.from[rank], 0) = s;
     if (cluster.num_blocks() > 1)
         cluster.sync();
     else
@@ -346,11 +524,11 @@ __device__ __noinline__ void perform(const Slice<T>& z, float max, Shared& sh) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
+__global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     extern __shared__ __align__(16) uint8_t dynamic[];
     __shared__ Shared sh;
     using View = RowView<T>;
-    constexpr uint32_t kPer = View::kPer, kVec = View::kVec, kChunk = View::kChunk;
+    constexpr uint32_t kVec = View::kVec;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t r = blockIdx.x / ctas, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -389,7 +567,9 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
     uint32_t* bin_n = reinterpret_cast<uint32_t*>(dynamic);                // kBins counts and
     uint32_t* bin_w = bin_n + kBins;                                       // kBins masses
     uint32_t* again = reinterpret_cast<uint32_t*>(list + kList);           // kChunks chunk numbers
-    double* tile_sum = reinterpret_cast<double*>(again + kChunks);         // a tile's
+    uint16_t* order = reinterpret_cast<uint16_t*>(again);                  // (later) the list's order
+    uint32_t* slots = again + kChunks;                                     // 2 kSlots words
+    double* tile_sum = reinterpret_cast<double*>(slots + 2 * kSlots);      // a tile's
     float* chunk_max = reinterpret_cast<float*>(tile_sum + (tiles + 1) / 2 * 2);
     double* first_sum = cluster.map_shared_rank(tile_sum, 0);
     float* first_max = cluster.map_shared_rank(chunk_max, 0);
@@ -407,16 +587,8 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
     for (uint32_t t = t0 + warp; t < t1; t += kWarps) {
         float v[32];
         row.tile(t, v);
-        float tile_top = -INFINITY, mine = 0.0f;
-#pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) {
-            float m = v[i * kVec];
-#pragma unroll
-            for (uint32_t e = 1; e < kVec; ++e) m = max_nan(m, v[i * kVec + e]);
-            m = warp_max_nan(m);
-            if (lane == i) mine = m;
-            tile_top = max_nan(tile_top, m);
-        }
+        float tile_top;
+        const float mine = row.chunk_max(v, &tile_top);
         if (lane < kPer) first_max[t * kPer + lane] = mine;
         top = max_nan(top, tile_top);
         if (!(by_mass || whole) || greedy) continue;
@@ -459,6 +631,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
         if (threadIdx.x < ctas) {
             uint32_t* o = cluster.map_shared_rank(sh.order, threadIdx.x);
             o[0] = op, o[1] = hi, o[2] = lo, o[3] = shift;
+            if (op == kCandidates) *cluster.map_shared_rank(&sh.bound, threadIdx.x) = sh.bound;
         }
         all_sync();
     };
@@ -491,12 +664,12 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
             if (chunk_max[i] == top) at = i;
         at = block_min(at, sh);
         if (warp == 0) {
-            float v[kVec];
-            const uint32_t j = at * kChunk + lane * kVec;
-            row.vec(j, v);
+            float v[4];
+            const uint32_t j = at * kChunk + lane * 4;
+            row.quad(j, v);
             uint32_t index = kAll;
 #pragma unroll
-            for (int e = (int)kVec - 1; e >= 0; --e)
+            for (int e = 3; e >= 0; --e)
                 if (v[e] == top) index = j + e - row.skew;
             index = __reduce_min_sync(kAll, index);
             if (lane == 0) finish(LRS_OK, index, 1.0, 1);
@@ -522,17 +695,19 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
     const double top_p = (double)p.top_p;
     double reach_lo = by_mass ? top_p * z * (1.0 - kApprox) : INFINITY, reach_hi = by_mass ? top_p * z * (1.0 + kApprox) : INFINITY;
 
-    // Sorted candidates (below `base` kept elements): how many of them are kept.
+    // Ordered candidates (below `base` kept elements): how many of them are kept.
     auto cut_list = [&](uint32_t count, const Sum& base, double reach_a, double reach_b, uint32_t* at_b) {
         const uint32_t per = (count + kThreads - 1) / kThreads;
         const uint32_t i0 = min(count, threadIdx.x * per), i1 = min(count, i0 + per);
         Sum s{0, 0.0, 0.0}, before;
-        for (uint32_t i = i0; i < i1; ++i) s.lo += weigh(value_of((uint32_t)(list[i] >> 32)));
+#pragma unroll 4
+        for (uint32_t i = i0; i < i1; ++i) s.lo += weigh(value_of((uint32_t)(list[order[i]] >> 32)));
         block_scan(s, &before, sh);
         double run = base.lo + before.lo;
         uint32_t a = 0, b = 0;
+#pragma unroll 4
         for (uint32_t i = i0; i < i1; ++i) {
-            const double w = weigh(value_of((uint32_t)(list[i] >> 32)));
+            const double w = weigh(value_of((uint32_t)(list[order[i]] >> 32)));
             const bool in = base.n + i < k && w >= (double)p.min_p;
             a += in && run < reach_a;
             b += in && run < reach_b;
@@ -542,120 +717,236 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
         *at_b = both.n >> 16;
         return both.n & 0xFFFFu;
     };
-    // The kept elements of the list, re-keyed and sorted by index.
-    auto by_index = [&](uint32_t count) {
-        for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
-            const uint64_t e = list[i];
-            list[i] = (uint64_t)~(uint32_t)e << 32 | e >> 32;
-        }
-        __syncthreads();
-        sort<false>(list, count);
-    };
+    auto units_of = [&](uint64_t entry) { return __double2ull_rn(weigh(value_of((uint32_t)(entry >> 32))) * 0x1p51); };
 
     if (!whole) {
         // ---- 2. few survivors ----
-        uint32_t bound = kLowest;
+        float least = value_of(kLowest);  // nothing lighter than min_p is kept
         if (p.min_p > 0.0f) {
             const double below = log2((double)p.min_p) / c;
-            const double x = (double)top + below - (fabs((double)top) - below) * 1e-12;
-            bound = max(bound, key_of(__double2float_rd(x)));
+            least = fmaxf(least, __double2float_rd((double)top + below - (fabs((double)top) - below) * 1e-12));
         }
-        // the largest key at which the chunk maxima alone fill top_k or top_p (no need to find it to the
-        // last bit: a few chunks more cost less than the steps)
-        auto filled = [&](uint32_t key, uint32_t* count) {
-            Sum s{0, 0.0, 0.0};
+        // How far below the maximum the list has to go: the chunk maxima alone fill top_k or top_p there.
+        uint32_t* few_n = reinterpret_cast<uint32_t*>(dynamic);  // counts of a bin
+        uint32_t* few_w = few_n + kThreads;                      // masses, in units that never round up
+        float low = top;
+        for (uint32_t i = threadIdx.x; i < chunks; i += kThreads)
+            if (chunk_max[i] >= least) low = fminf(low, chunk_max[i]);
+        low = block_min_float(low, sh);
+        const uint32_t unit = min(mass_unit(chunks), 1u << 24);
+        const uint64_t mass_goal = by_mass ? __double2ull_ru(fmin(reach_hi * unit, 0x1p40)) : ~0ull;
+        Bound bound{top, low < top ? fminf(255.9f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f, least, 0.0f, 1e30f, true};  // (halves: no overflow)
+        uint32_t reaching = 0;
+        for (int round = 0; round < 2; ++round) {
+            few_n[threadIdx.x] = 0, few_w[threadIdx.x] = 0;
+            __syncthreads();
+            uint32_t above = 0, above_w = 0;
             for (uint32_t i = threadIdx.x; i < chunks; i += kThreads) {
                 const float m = chunk_max[i];
-                if (key_of(m) >= key) {
-                    ++s.n;
-                    if (by_mass) s.lo += weigh(m);
+                if (!(m >= least)) continue;
+                float f = bound.distance(m);
+                const uint32_t w = by_mass ? __double2uint_rd(weigh(m) * unit) : 0u;
+                if (round == 1) {
+                    if (f < bound.edge0 - 1.0f) above += 1, above_w += w;
+                    if (!(f >= bound.edge0 - 1.0f && f < bound.edge0)) continue;
+                    f = (f - (bound.edge0 - 1.0f)) * 256.0f;
                 }
+                const uint32_t b = min((uint32_t)f, kThreads - 1);
+                atomicAdd(&few_n[b], 1u);
+                if (by_mass) atomicAdd(&few_w[b], w);
             }
-            s = block_scan(s, nullptr, sh);
-            *count = s.n;
-            return s.n >= k || s.lo >= reach_hi;
-        };
-        uint32_t reaching;
-        if (filled(bound, &reaching)) {
-            uint32_t lo = bound, hi = key_of(top) + 1;
-            while (hi - lo > 1 && reaching > (k < chunks ? k + 32 : 64)) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                uint32_t count;
-                if (filled(mid, &count))
-                    lo = mid, reaching = count;
-                else
-                    hi = mid;
+            if (above) atomicAdd(&few_n[0], above), atomicAdd(&few_w[0], above_w);  // (counted with the first bin)
+            __syncthreads();
+            const uint32_t bin = threadIdx.x;
+            uint32_t before_n, before_w;
+            block_scan_words(few_n[bin], few_w[bin], &before_n, &before_w, sh);
+            const uint32_t upto = before_n + few_n[bin];
+            const bool fills = upto >= k || (uint64_t)before_w + few_w[bin] >= mass_goal;
+            const uint32_t at = block_min(fills ? bin : kAll, sh);
+            if (at == kAll) {  // not even all of them: every element from `least` up
+                bound.bounded = false;
+                break;
             }
-            bound = lo;
+            if (bin == at) sh.count = upto;
+            __syncthreads();
+            reaching = sh.count;
+            if (round == 0)
+                bound.edge0 = (float)(at + 1);
+            else
+                bound.edge1 = (float)(at + 1);
+            if (reaching <= (k < chunks ? k + 32 : 64)) break;
+            __syncthreads();
         }
         __syncthreads();
-        if (threadIdx.x == 0) sh.count = 0, sh.chunks = 0;
+        if (threadIdx.x == 0) sh.count = 0, sh.chunks = 0, sh.bound = bound;
         __syncthreads();
+        for (uint32_t i = threadIdx.x; i < chunks; i += kThreads) {
+            if (!bound(chunk_max[i])) continue;
+            const uint32_t at = atomicAdd(&sh.chunks, 1u);
+            if (at < kChunks) again[at] = i;
+        }
+        __syncthreads();
+        reaching = sh.chunks;
         if (reaching <= kChunks) {
-            for (uint32_t i = threadIdx.x; i < chunks; i += kThreads)
-                if (key_of(chunk_max[i]) >= bound) again[atomicAdd(&sh.chunks, 1u)] = i;
-            __syncthreads();
-            constexpr uint32_t kAtOnce = 16 / kVec;
-            for (uint32_t i = warp * kAtOnce; i < reaching; i += kWarps * kAtOnce) {
-                float v[kAtOnce][kVec];
+            if (ctas > 1 && reaching > kWarps * 8) {  // many chunks: all CTAs, each its slice
+                command(kCandidates, 0, 0, 0);
+                perform(slice, top, sh);
+            } else {
+                for (uint32_t i = warp * 8; i < reaching; i += kWarps * 8) {
+                    float v[32];
+                    uint32_t from[8], mask = 0;
 #pragma unroll
-                for (uint32_t q = 0; q < kAtOnce; ++q)
-                    if (i + q < reaching) row.vec(again[i + q] * kChunk + lane * kVec, v[q]);
-#pragma unroll
-                for (uint32_t q = 0; q < kAtOnce; ++q) {
-                    if (i + q >= reaching) break;
-                    const uint32_t j = again[i + q] * kChunk + lane * kVec - row.skew;
-#pragma unroll
-                    for (uint32_t e = 0; e < kVec; ++e) {
-                        const uint32_t key = key_of(v[q][e]);
-                        const uint32_t vote = __ballot_sync(kAll, key >= bound);
-                        if (vote == 0) continue;
-                        uint32_t at = 0;
-                        if (lane == 0) at = atomicAdd(&sh.count, __popc(vote));
-                        at = __shfl_sync(kAll, at, 0) + __popc(vote & ((1u << lane) - 1));
-                        if (key >= bound && at < kList) list[at] = (uint64_t)key << 32 | ~(j + e);
+                    for (uint32_t q = 0; q < 8; ++q) {
+                        from[q] = i + q < reaching ? again[i + q] * kChunk + lane * 4 : row.end;
+                        row.quad(from[q], *reinterpret_cast<float(*)[4]>(&v[4 * q]));
                     }
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) mask |= bound(v[q]) ? 1u << q : 0u;
+                    append<T>(list, &sh.count, v, mask, [&](int q) { return from[q / 4] + q % 4 - row.skew; });
                 }
             }
             __syncthreads();
             const uint32_t count = sh.count;
-            if (count <= kList) {
-                sort<true>(list, count);
-                uint32_t other;
-                uint32_t keep = cut_list(count, Sum{0, 0.0, 0.0}, reach_lo, reach_hi, &other);
-                if (keep != other) {  // Z's error decides: the row's mass again, in 64 bits
-                    Sum s{0, 0.0, 0.0};
-                    for (uint32_t t = warp; t < tiles; t += kWarps) {
-                        float v[32];
-                        row.tile(t, v);
+            auto row_mass = [&] {  // Z again, in 64 bits
+                Sum s{0, 0.0, 0.0};
+                for (uint32_t t = warp; t < tiles; t += kWarps) {
+                    float v[32];
+                    row.tile(t, v);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s.lo += weigh(v[i]);
+                    for (int i = 0; i < 32; ++i) s.lo += weigh(v[i]);
+                }
+                return block_scan(s, nullptr, sh).lo;
+            };
+            if (count <= kFew) {
+                // Every candidate's rank and the mass before it by comparison with all, the comparisons of
+                // one shared by `lanes` neighbours; masses are whole numbers of 2^-51, so that their sums do
+                // not depend on the list's order.
+                uint32_t lanes = 1;
+                while (lanes < 32 && count * lanes * 2 <= kThreads) lanes *= 2;
+                const uint32_t me = threadIdx.x / lanes, part = threadIdx.x % lanes;
+                const bool real = me < count;
+                uint64_t* mass = list + kFew;   // of every candidate
+                const uint64_t entry = real ? list[me] : 0;
+                const double w = real ? weigh(value_of((uint32_t)(entry >> 32))) : 0.0;
+                const uint64_t units = __double2ull_rn(w * 0x1p51);
+                if (real && part == 0) mass[me] = units;
+                __syncthreads();
+                uint32_t rank = 0;
+                uint64_t before = 0;
+                if (real)
+                    for (uint32_t j = part; j < count; j += lanes) {
+                        const bool over = list[j] > entry;
+                        rank += over;
+                        before += over ? mass[j] : 0;
                     }
-                    z = block_scan(s, nullptr, sh).lo;
-                    keep = cut_list(count, Sum{0, 0.0, 0.0}, top_p * z, top_p * z, &other);
+                for (uint32_t o = 1; o < lanes; o *= 2) {
+                    rank += __shfl_xor_sync(kAll, rank, o);
+                    before += __shfl_xor_sync(kAll, before, o);
                 }
-                by_index(keep);
-                const uint32_t per = (keep + kThreads - 1) / kThreads;
-                const uint32_t i0 = min(keep, threadIdx.x * per), i1 = min(keep, i0 + per);
-                Sum s{0, 0.0, 0.0}, before;
-                for (uint32_t i = i0; i < i1; ++i) s.lo += weigh(value_of((uint32_t)list[i]));
-                const double mass = block_scan(s, &before, sh).lo, target = (double)u * mass;
-                uint32_t found = kAll;
-                double run = before.lo;
-                for (uint32_t i = i0; i < i1; ++i) {
-                    run += weigh(value_of((uint32_t)list[i]));
-                    if (run > target) {
-                        found = i;
-                        break;
+                auto kept_to = [&](double reach) {
+                    return real && rank < k && w >= (double)p.min_p && (!by_mass || before < __double2ull_ru(fmin(reach * 0x1p51, 0x1p63)));
+                };
+                bool keep = kept_to(reach_lo);
+                if (__syncthreads_or(keep != kept_to(reach_hi))) {  // Z's error decides
+                    z = row_mass();
+                    keep = kept_to(top_p * z);
+                }
+                if (real && part == 0) mass[me] = keep ? units : 0;
+                const uint32_t kept = __syncthreads_count(keep && part == 0);
+                const uint32_t index = ~(uint32_t)entry;
+                uint64_t upto = 0, total = 0;
+                if (real)
+                    for (uint32_t j = part; j < count; j += lanes) {
+                        const uint64_t m = mass[j];
+                        total += m;
+                        upto += ~(uint32_t)list[j] <= index ? m : 0;
                     }
+                for (uint32_t o = 1; o < lanes; o *= 2) {
+                    total += __shfl_xor_sync(kAll, total, o);
+                    upto += __shfl_xor_sync(kAll, upto, o);
                 }
-                found = block_min(found, sh);
-                if (threadIdx.x == 0) {
-                    if (found == kAll)  // (two orders of a sum: the last weight, when none passes the target)
-                        for (found = keep - 1; found > 0 && weigh(value_of((uint32_t)list[found])) == 0.0;) --found;
-                    const uint64_t e = list[found];
-                    finish(LRS_OK, (uint32_t)(e >> 32), weigh(value_of((uint32_t)e)) / mass, keep);
+                const bool passes = keep && units && (double)upto > (double)u * (double)total;
+                uint32_t token = block_min(passes ? index : kAll, sh);
+                if (token == kAll) token = ~block_min(keep && units ? ~index : kAll, sh);  // (u's product rounded up: the last)
+                if (real && part == 0 && index == token) finish(LRS_OK, token, w * 0x1p51 / (double)total, kept);
+                return leave();
+            }
+            if (count <= kList) {
+                uint64_t cut = 0;  // the last entry kept
+                uint32_t keep = count;
+                if (by_mass || k < count) {
+                    rank_list(list, order, slots, count, sh);
+                    uint32_t other;
+                    keep = cut_list(count, Sum{0, 0.0, 0.0}, reach_lo, reach_hi, &other);
+                    if (keep != other) {  // Z's error decides
+                        z = row_mass();
+                        keep = cut_list(count, Sum{0, 0.0, 0.0}, top_p * z, top_p * z, &other);
+                    }
+                    cut = list[order[keep - 1]];
+                } else if (p.min_p > 0.0f) {
+                    uint32_t mine = 0;
+                    for (uint32_t i = threadIdx.x; i < count; i += kThreads)
+                        if (weigh(value_of((uint32_t)(list[i] >> 32))) >= (double)p.min_p)
+                            ++mine;
+                        else
+                            list[i] = 0;
+                    keep = block_scan(Sum{mine, 0.0, 0.0}, nullptr, sh).n;
+                    cut = 1;
                 }
+                // The token: masses (whole numbers of 2^-51: their sums know no order) by ranges of indices,
+                // the range that the target falls in again by parts where it is crowded, then its entries.
+                uint64_t* range = reinterpret_cast<uint64_t*>(slots);
+                uint32_t first = 0, width = (n + kSlots - 1) / kSlots;  // indices from `first`, `width` a range
+                uint64_t below = 0, total = 0;
+                double target = 0.0;
+                for (int round = 0; round < 2; ++round) {
+                    __syncthreads();
+                    for (uint32_t i = threadIdx.x; i < kSlots; i += kThreads) range[i] = 0;
+                    if (threadIdx.x == 0) sh.count = 0;
+                    __syncthreads();
+#pragma unroll 4
+                    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+                        const uint64_t e = list[i];
+                        const uint32_t slot = (~(uint32_t)e - first) / width;  // (before `first`: out of range too)
+                        if (e >= cut && slot < kSlots) atomicAdd(reinterpret_cast<unsigned long long*>(&range[slot]), units_of(e));
+                    }
+                    __syncthreads();
+                    const uint64_t a = range[2 * threadIdx.x], b = range[2 * threadIdx.x + 1];
+                    uint64_t before;
+                    const uint64_t all = block_scan_long(a + b, &before, sh);
+                    before += below;
+                    if (round == 0) total = all, target = (double)u * (double)total;
+                    uint32_t hit = (double)(before + a) > target ? 2 * threadIdx.x : (double)(before + a + b) > target ? 2 * threadIdx.x + 1 : kAll;
+                    hit = block_min(hit, sh);
+                    if (hit == kAll) hit = ~block_min(b ? ~(2 * threadIdx.x + 1) : a ? ~(2 * threadIdx.x) : kAll, sh);  // (u's product rounded up: the last)
+                    if (threadIdx.x == hit / 2) sh.cut = hit % 2 ? before + a : before;
+                    __syncthreads();
+                    below = sh.cut;
+                    first += hit * width;
+                    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+                        const uint64_t e = list[i];
+                        if (e < cut || ~(uint32_t)e - first >= width) continue;
+                        const uint32_t at = atomicAdd(&sh.count, 1u);
+                        if (at < kThreads) again[at] = i;
+                    }
+                    __syncthreads();
+                    if (sh.count <= kThreads) break;
+                    width = (width + kSlots - 1) / kSlots;  // (at most 2^22 / 512 / 512 = 16 indices then)
+                }
+                const uint32_t members = sh.count;
+                const uint64_t entry = threadIdx.x < members ? list[again[threadIdx.x]] : 0;
+                const uint32_t index = ~(uint32_t)entry;
+                uint64_t upto = below;
+                if (entry)
+                    for (uint32_t j = 0; j < members; ++j) {
+                        const uint64_t e = list[again[j]];
+                        if (~(uint32_t)e <= index) upto += units_of(e);
+                    }
+                const bool weighs = entry && units_of(entry);
+                uint32_t token = block_min(weighs && (double)upto > target ? index : kAll, sh);
+                if (token == kAll) token = ~block_min(weighs ? ~index : kAll, sh);
+                if (entry && index == token)
+                    finish(LRS_OK, token, weigh(value_of((uint32_t)(entry >> 32))) * 0x1p51 / (double)total, keep);
                 return leave();
             }
         }
@@ -685,15 +976,12 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
             const uint32_t range = hi - lo;
             const uint32_t bits = 32 - __clz(range - 1 | 1);
             const uint32_t shift = bits > 12 ? bits - 12 : 0;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads) bin_n[i] = 0;
             command(kHistogram, hi, lo, shift);
             perform(slice, top, sh);
             base = total();
             if (by_mass) reach = top_p * base.hi;
-            for (uint32_t q = 1; q < ctas; ++q) {
-                const uint32_t* other = cluster.map_shared_rank(bin_n, q);
-                for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads) bin_n[i] += other[i];
-            }
-            __syncthreads();
             // where the cut may lie: counts are exact, masses within their rounding (half a unit an
             // element, and the 32-bit power)
             constexpr uint32_t kEach = kBins / kThreads;
@@ -704,7 +992,8 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
                 if (m == 0 || !by_mass) return 0.0;
                 const float y = (value_of(hi - 1 - (b << shift)) - top) * cf;
                 const double err = 0x1p-20 * (2.0 + fabs((double)y));
-                const double s = unit * power2(fmax((double)ceilf(y), -2000.0));
+                const int up = (int)fmaxf(ceilf(y), -900.0f);  // (a bin that far below weighs nothing)
+                const double s = unit * (up > -900 ? __hiloint2double((1023 + up) << 20, 0) : 0.0);
                 return upper ? ((double)w + m) * s * (1.0 + err) : fmax(0.0, ((double)w - m) * s * (1.0 - err));
             };
             Sum s{0, 0.0, 0.0}, before;
@@ -784,28 +1073,20 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
             }
         } else {
             const uint32_t count = min(sh.count, kList);
-            sort<true>(list, count);
+            rank_list(list, order, slots, count, sh);
             uint32_t other;
             const uint32_t keep = cut_list(count, above, reach, reach, &other);
-            cut = keep ? list[keep - 1] : (uint64_t)hi << 32;
+            cut = keep ? list[order[keep - 1]] : (uint64_t)hi << 32;
             kept = above.n + keep;
+            // (the chunks' maxima have served: each tile's share of the list, in units whose sums know no order)
+            uint64_t* share = reinterpret_cast<uint64_t*>(chunk_max);
+            for (uint32_t t = threadIdx.x; t < tiles; t += kThreads) share[t] = 0;
             __syncthreads();
-            by_index(keep);
-            for (uint32_t t = threadIdx.x; t < tiles; t += kThreads) {
-                const uint32_t from = t * kTile < row.skew ? 0 : t * kTile - row.skew;  // the tile's first index
-                uint32_t a = 0, b = keep;
-                while (a < b) {
-                    const uint32_t mid = (a + b) / 2;
-                    if ((uint32_t)(list[mid] >> 32) < from)
-                        a = mid + 1;
-                    else
-                        b = mid;
-                }
-                double w = tile_sum[t];
-                for (; a < keep && (uint32_t)(list[a] >> 32) < (t + 1) * kTile - row.skew; ++a)
-                    w += weigh(value_of((uint32_t)list[a]));
-                tile_sum[t] = w;
-            }
+            for (uint32_t i = threadIdx.x; i < count; i += kThreads)
+                if (list[i] >= cut)
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&share[(~(uint32_t)list[i] + row.skew) / kTile]), units_of(list[i]));
+            __syncthreads();
+            for (uint32_t t = threadIdx.x; t < tiles; t += kThreads) tile_sum[t] += (double)share[t] * 0x1p-51;
         }
     }
     leave();
@@ -837,10 +1118,10 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args g) {
         const uint32_t quota = tie_keep ? reinterpret_cast<uint32_t*>(chunk_max)[tile] : 0;
         uint32_t seen = 0, token = kAll, final = kAll;
         double w_token = 0.0, w_final = 0.0;
-        for (uint32_t i = 0; i < kPer && token == kAll; ++i) {
+        for (uint32_t i = 0; i < View::kLoads && token == kAll; ++i) {
             float v[kVec];
             double w[kVec], sum = 0.0;
-            const uint32_t j = tile * kTile + i * kChunk + lane * kVec;
+            const uint32_t j = tile * kTile + i * View::kLoad + lane * kVec;
             row.vec(j, v);
             uint32_t tied = 0;
 #pragma unroll
@@ -902,7 +1183,7 @@ constexpr int kMaxDevices = 64;
 template <typename T>
 size_t shared_bytes(uint32_t n) {
     const uint32_t tiles = (n + 15 + kTile - 1) / kTile;
-    return kList * 8 + kChunks * 4 + (tiles + 1) / 2 * 2 * 8 + (size_t)tiles * RowView<T>::kPer * 4;
+    return kList * 8 + kChunks * 4 + kSlots * 8 + (tiles + 1) / 2 * 2 * 8 + (size_t)tiles * kPer * 4;
 }
 
 template <typename T>
@@ -922,10 +1203,10 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
         if (e != cudaSuccess) return lrs_call_error(LRS_E_CUDA, "lrs_draw_device: %s", cudaGetErrorString(e));
         sms[dev] = count;
     }
-    // CTAs a row: as many as fill two an SM, no more than give each warp a tile
+    // CTAs a row: as many as fill four an SM, no more than give each warp a tile
     const uint32_t tiles = (g.n + 15 + kTile - 1) / kTile;
     uint32_t ctas = 1;
-    while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 2 * (uint64_t)sms[dev] && ctas * kWarps < tiles) ctas *= 2;
+    while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 4 * (uint64_t)sms[dev] && ctas * kWarps < tiles) ctas *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(rows * ctas);
     cfg.blockDim = dim3(kThreads);

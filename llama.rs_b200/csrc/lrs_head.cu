@@ -404,17 +404,19 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
         bool ok = true;
         for (uint32_t t = blockIdx.x; t < g.tiles; t += gridDim.x) {
             const uint32_t r0 = t % g.row_tiles * kWideR + quarter * 32, v0 = t / g.row_tiles * kWideV + c0;
-            // the scales of this thread's row and of its columns' weights, a step ahead of their use
+            // the scales of this thread's row and of its columns' weights, two steps ahead of their use
             const float* sa = g.sa + min(r0 + lane, g.rows - 1);
             const float* sw = g.sw + min(v0, g.n - 1) / kBlock * g.ld_ws;
-            float a1 = __ldg(sa), w1 = __ldg(sw);
+            float a0 = __ldg(sa), w0 = __ldg(sw), a1 = a0, w1 = w0;
+            if (g.blocks > 1) sa += g.ld_as, ++sw, a1 = __ldg(sa), w1 = __ldg(sw);
             float acc[kWideCols];
 #pragma unroll
             for (int i = 0; i < (int)kWideCols; ++i) acc[i] = 0.0f;
             // (after a wait that ran out the steps go on without waiting, and the tile is lost)
             for (uint32_t b = 0; b < g.blocks; ++b) {
-                const float s0 = a1 * w1;
-                if (b + 1 < g.blocks) sa += g.ld_as, ++sw, a1 = __ldg(sa), w1 = __ldg(sw);
+                const float s0 = a0 * w0;
+                a0 = a1, w0 = w1;
+                if (b + 2 < g.blocks) sa += g.ld_as, ++sw, a1 = __ldg(sa), w1 = __ldg(sw);
                 ok &= bar_wait(tfull + buffer * 8, turn, lost);
                 __syncwarp();
                 tmem_fence_after();
