@@ -225,6 +225,17 @@ __device__ __noinline__ void sort(uint64_t* list, uint32_t count) {
     __syncthreads();
 }
 
+// Sums of up to 2^12 whole numbers of up to 2^51 in three words of 17 bits each (32-bit additions to shared
+// memory are the ones that the hardware does in place).
+__device__ __forceinline__ void add_units(uint32_t* sum, uint64_t units) {
+    atomicAdd(sum, (uint32_t)units & 0x1FFFFu);
+    atomicAdd(sum + 1, (uint32_t)(units >> 17) & 0x1FFFFu);
+    atomicAdd(sum + 2, (uint32_t)(units >> 34));
+}
+__device__ __forceinline__ uint64_t read_units(const uint32_t* sum) {
+    return sum[0] + ((uint64_t)sum[1] << 17) + ((uint64_t)sum[2] << 34);
+}
+
 constexpr uint32_t kSlots = 512;  // of the bins below
 constexpr uint32_t kOwn = kList / kThreads;
 
@@ -430,8 +441,7 @@ __device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const fl
     }
 }
 
-// One operation of the first CTA's over this CTA's slice of the row: keys from `hi` up are summed, those
-// of [lo, hi) counted by bin, listed, or counted by tile.
+// What every CTA does with its slice of the row when the first CTA says so (sh.order).
 template <typename T>
 struct Slice {
     RowView<T> row;
@@ -440,62 +450,94 @@ struct Slice {
     uint8_t* dynamic;    // (as the kernel lays it out)
     double* first_sum;
     float* first_max;
+    __device__ __forceinline__ uint32_t index(uint32_t t, int i) const {  // of element i of a lane's 32
+        return t * kTile + i / RowView<T>::kVec * RowView<T>::kLoad + threadIdx.x % 32 * RowView<T>::kVec + i % RowView<T>::kVec - row.skew;
+    }
 };
 
+// Candidates: the elements that pass the bound, to the first CTA's list.
 template <typename T>
-__device__ __noinline__ void perform(const Slice<T>& z, float max, Shared& sh) {
-    using View = RowView<T>;
+__device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const uint32_t op = sh.order[0], hi = sh.order[1], lo = sh.order[2], shift = sh.order[3];
-    uint32_t* bin_n = reinterpret_cast<uint32_t*>(z.dynamic);
-    uint32_t* bin_w = bin_n + kBins;
     uint64_t* first_list = cluster.map_shared_rank(reinterpret_cast<uint64_t*>(z.dynamic), 0);
     uint32_t* first_count = cluster.map_shared_rank(&sh.count, 0);
-    const Weigh weigh{(double)max, z.c};
-    const float cf = (float)z.c, scale = (float)mass_unit(z.n);
-    Sum s{0, 0.0, 0.0};  // elements from hi up: count and mass; mass of all (histograms)
     const Bound bound = sh.bound;
+    for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
+        float v[32];
+        z.row.tile(t, v);
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mask |= bound(v[i]) ? 1u << i : 0u;
+        append<T>(first_list, first_count, v, mask, [&](int i) { return z.index(t, i); });
+    }
+}
+
+// The upper end of a bin's weights as a power of two, 2^edge.
+__device__ __forceinline__ float bin_edge(uint32_t key, float max, float c) { return ceilf((value_of(key) - max) * c); }
+
+// Counts and masses of the keys of [lo, hi) in bins of 2^shift keys, the highest first, to the first CTA's
+// bins (clear before); returns the count and mass (64 bits) of the keys above.
+template <typename T>
+__device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t hi = sh.order[1], lo = sh.order[2], shift = sh.order[3];
+    uint32_t* bin_n = reinterpret_cast<uint32_t*>(z.dynamic);
+    uint32_t* bin_w = bin_n + kBins;
     const uint32_t rank = cluster.block_rank();
-    if (op == kHistogram && rank) {  // (the first CTA's bins are clear: the others' come to them)
+    if (rank) {
         for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads) bin_n[i] = 0;
         __syncthreads();
     }
-    for (uint32_t t = z.t0 + warp; t < z.t1; t += kWarps) {
+    const Weigh weigh{(double)max, z.c};
+    const float cf = (float)z.c, scale = (float)mass_unit(z.n);
+    Sum s{0, 0.0, 0.0};
+    for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
         float v[32];
         z.row.tile(t, v);
-        double above = 0.0;
-        if (op == kHistogram) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const uint32_t key = key_of(v[i]);
-                const double w = weigh(v[i]);
-                s.hi += w;
-                if (key >= hi) {
-                    s.lo += w, ++s.n;
-                } else if (key >= lo) {
-                    const uint32_t b = (hi - 1 - key) >> shift;
-                    const float edge = ceilf((value_of(hi - 1 - (b << shift)) - max) * cf);
-                    float e;
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v[i] - max) * cf - edge));
-                    atomicAdd(&bin_n[b], 1u);
-                    atomicAdd(&bin_w[b], __float2uint_rn(fminf(e, 2.0f) * scale));
-                }
-            }
-            continue;
-        }
-        auto index = [&](int i) { return t * kTile + i / View::kVec * View::kLoad + lane * View::kVec + i % View::kVec - z.row.skew; };
-        uint32_t mask = 0;
-        if (op == kCandidates) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mask |= bound(v[i]) ? 1u << i : 0u;
-            append<T>(first_list, first_count, v, mask, index);
-            continue;
-        }
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const uint32_t key = key_of(v[i]);
-            if (key >= hi) above += weigh(v[i]), ++s.n;
+            if (key >= hi) {
+                s.lo += weigh(v[i]), ++s.n;
+            } else if (key >= lo) {
+                const uint32_t b = (hi - 1 - key) >> shift;
+                float e;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v[i] - max) * cf - bin_edge(hi - 1 - (b << shift), max, cf)));
+                atomicAdd(&bin_n[b], 1u);
+                atomicAdd(&bin_w[b], __float2uint_rn(fminf(e, 2.0f) * scale));
+            }
+        }
+    }
+    if (rank) {
+        __syncthreads();
+        uint32_t* first_bin = cluster.map_shared_rank(bin_n, 0);
+        for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads)
+            if (bin_n[i]) atomicAdd(&first_bin[i], bin_n[i]);
+    }
+    return s;
+}
+
+// Sums in 64 bits of the keys from hi up and of all, by tile as well (kSumAbove: not by tile); the keys
+// of [lo, hi) go to the first CTA's list, or (kGatherTies) are counted by tile.
+template <typename T>
+__device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t op = sh.order[0], hi = sh.order[1], lo = sh.order[2], lane = threadIdx.x % 32;
+    uint64_t* first_list = cluster.map_shared_rank(reinterpret_cast<uint64_t*>(z.dynamic), 0);
+    uint32_t* first_count = cluster.map_shared_rank(&sh.count, 0);
+    const Weigh weigh{(double)max, z.c};
+    Sum s{0, 0.0, 0.0};
+    for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
+        float v[32];
+        z.row.tile(t, v);
+        double above = 0.0;
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t key = key_of(v[i]);
+            const double w = weigh(v[i]);
+            s.hi += w;
+            if (key >= hi) above += w, ++s.n;
             mask |= key >= lo && key < hi ? 1u << i : 0u;
         }
         s.lo += above;
@@ -506,17 +548,23 @@ __device__ __noinline__ void perform(const Slice<T>& z, float max, Shared& sh) {
             const uint32_t ties = __reduce_add_sync(kAll, __popc(mask));
             if (lane == 0) reinterpret_cast<uint32_t*>(z.first_max)[t] = ties;
         } else {
-            append<T>(first_list, first_count, v, mask, index);
+            append<T>(first_list, first_count, v, mask, [&](int i) { return z.index(t, i); });
         }
     }
-    if (op == kHistogram && rank) {
-        __syncthreads();
-        uint32_t* first_bin = cluster.map_shared_rank(bin_n, 0);
-        for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads)
-            if (bin_n[i]) atomicAdd(&first_bin[i], bin_n[i]);
-    }
+    return s;
+}
+
+template <typename T>
+__device__ void perform(const Slice<T>& z, float max, Shared& sh) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t op = sh.order[0];
+    Sum s{0, 0.0, 0.0};
+    if (op == kCandidates)
+        list_candidates(z, sh);
+    else
+        s = op == kHistogram ? histogram(z, max, sh) : gather(z, max, sh);
     s = block_scan(s, nullptr, sh);
-    if (threadIdx.x == 0) *cluster.map_shared_rank(&sh.from[rank], 0) = s;
+    if (threadIdx.x == 0) *cluster.map_shared_rank(&sh.from[cluster.block_rank()], 0) = s;
     if (cluster.num_blocks() > 1)
         cluster.sync();
     else
@@ -527,8 +575,6 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     extern __shared__ __align__(16) uint8_t dynamic[];
     __shared__ Shared sh;
-    using View = RowView<T>;
-    constexpr uint32_t kVec = View::kVec;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t r = blockIdx.x / ctas, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -568,8 +614,8 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     uint32_t* bin_w = bin_n + kBins;                                       // kBins masses
     uint32_t* again = reinterpret_cast<uint32_t*>(list + kList);           // kChunks chunk numbers
     uint16_t* order = reinterpret_cast<uint16_t*>(again);                  // (later) the list's order
-    uint32_t* slots = again + kChunks;                                     // 2 kSlots words
-    double* tile_sum = reinterpret_cast<double*>(slots + 2 * kSlots);      // a tile's
+    uint32_t* slots = again + kChunks;                                     // 3 kSlots words
+    double* tile_sum = reinterpret_cast<double*>(slots + 3 * kSlots);      // a tile's
     float* chunk_max = reinterpret_cast<float*>(tile_sum + (tiles + 1) / 2 * 2);
     double* first_sum = cluster.map_shared_rank(tile_sum, 0);
     float* first_max = cluster.map_shared_rank(chunk_max, 0);
@@ -786,7 +832,8 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             if (at < kChunks) again[at] = i;
         }
         __syncthreads();
-        reaching = sh.chunks;
+        // (without a bound the list would be the row)
+        reaching = bound.bounded || p.min_p > 0.0f || n <= kList ? sh.chunks : kAll;
         if (reaching <= kChunks) {
             if (ctas > 1 && reaching > kWarps * 8) {  // many chunks: all CTAs, each its slice
                 command(kCandidates, 0, 0, 0);
@@ -895,23 +942,23 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 }
                 // The token: masses (whole numbers of 2^-51: their sums know no order) by ranges of indices,
                 // the range that the target falls in again by parts where it is crowded, then its entries.
-                uint64_t* range = reinterpret_cast<uint64_t*>(slots);
+                uint32_t* range = slots;  // three words each
                 uint32_t first = 0, width = (n + kSlots - 1) / kSlots;  // indices from `first`, `width` a range
                 uint64_t below = 0, total = 0;
                 double target = 0.0;
                 for (int round = 0; round < 2; ++round) {
                     __syncthreads();
-                    for (uint32_t i = threadIdx.x; i < kSlots; i += kThreads) range[i] = 0;
+                    for (uint32_t i = threadIdx.x; i < 3 * kSlots; i += kThreads) range[i] = 0;
                     if (threadIdx.x == 0) sh.count = 0;
                     __syncthreads();
 #pragma unroll 4
                     for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
                         const uint64_t e = list[i];
                         const uint32_t slot = (~(uint32_t)e - first) / width;  // (before `first`: out of range too)
-                        if (e >= cut && slot < kSlots) atomicAdd(reinterpret_cast<unsigned long long*>(&range[slot]), units_of(e));
+                        if (e >= cut && slot < kSlots) add_units(range + 3 * slot, units_of(e));
                     }
                     __syncthreads();
-                    const uint64_t a = range[2 * threadIdx.x], b = range[2 * threadIdx.x + 1];
+                    const uint64_t a = read_units(range + 6 * threadIdx.x), b = read_units(range + 6 * threadIdx.x + 3);
                     uint64_t before;
                     const uint64_t all = block_scan_long(a + b, &before, sh);
                     before += below;
@@ -970,8 +1017,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         }
         if (hi <= lo) lo = hi - 1;
         uint32_t inside = kAll;  // elements of [lo, hi)
-        Sum base{0, 0.0, 0.0};
-        double reach = INFINITY;
+        Sum base{0, 0.0, 0.0};   // count and mass from hi up
         for (int round = 0; round < 3 && inside > kList && (hi - lo > 1 || round == 0); ++round) {
             const uint32_t range = hi - lo;
             const uint32_t bits = 32 - __clz(range - 1 | 1);
@@ -981,34 +1027,32 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             command(kHistogram, hi, lo, shift);
             perform(slice, top, sh);
             base = total();
-            if (by_mass) reach = top_p * base.hi;
             // where the cut may lie: counts are exact, masses within their rounding (half a unit an
-            // element, and the 32-bit power)
+            // element, and the 32-bit power), Z within its own
             constexpr uint32_t kEach = kBins / kThreads;
             const float cf = (float)c;
             const double unit = 1.0 / (double)mass_unit(n);
-            auto mass = [&](uint32_t b, bool upper) {
+            auto step = [&](uint32_t b, Sum* run) {  // adds bin b
                 const uint32_t w = bin_w[b], m = bin_n[b];
-                if (m == 0 || !by_mass) return 0.0;
-                const float y = (value_of(hi - 1 - (b << shift)) - top) * cf;
-                const double err = 0x1p-20 * (2.0 + fabs((double)y));
-                const int up = (int)fmaxf(ceilf(y), -900.0f);  // (a bin that far below weighs nothing)
-                const double s = unit * (up > -900 ? __hiloint2double((1023 + up) << 20, 0) : 0.0);
-                return upper ? ((double)w + m) * s * (1.0 + err) : fmax(0.0, ((double)w - m) * s * (1.0 - err));
+                run->n += m;
+                if (m == 0 || !by_mass) return;
+                const uint32_t key = hi - 1 - (b << shift);
+                const float up = bin_edge(key, top, cf);
+                if (up < -900.0f) return;  // (weighs nothing)
+                const double s = unit * __hiloint2double((1023 + (int)up) << 20, 0);
+                const double err = 0x1p-20 * (3.0 - (double)up);
+                run->lo += fmax(0.0, ((double)w - m) * s * (1.0 - err)), run->hi += ((double)w + m) * s * (1.0 + err);
             };
             Sum s{0, 0.0, 0.0}, before;
-            for (uint32_t i = 0; i < kEach; ++i) {
-                const uint32_t b = threadIdx.x * kEach + i;
-                s.n += bin_n[b], s.lo += mass(b, false), s.hi += mass(b, true);
-            }
+            for (uint32_t i = 0; i < kEach; ++i) step(threadIdx.x * kEach + i, &s);
             block_scan(s, &before, sh);
             Sum run{base.n + before.n, base.lo + before.lo, base.lo + before.hi};
             uint32_t a = kBins - 1, z1 = kBins - 1;
             for (uint32_t i = 0; i < kEach; ++i) {
                 const uint32_t b = threadIdx.x * kEach + i;
-                run.n += bin_n[b], run.lo += mass(b, false), run.hi += mass(b, true);
-                if ((run.n >= k || run.hi >= reach) && b < a) a = b;
-                if ((run.n >= k || run.lo >= reach) && b < z1) z1 = b;
+                step(b, &run);
+                if ((run.n >= k || run.hi >= reach_lo) && b < a) a = b;
+                if ((run.n >= k || run.lo >= reach_hi) && b < z1) z1 = b;
             }
             a = block_min(a, sh), z1 = block_min(z1, sh);
             const uint32_t last = (range - 1) >> shift;
@@ -1021,22 +1065,25 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             lo = max(lo, from - min(from, (z1 + 1) << shift));
         }
         // (histograms that do not settle, as with a mass far below their unit: halves, summed exactly)
-        while (inside > kList && hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            command(kSumAbove, mid, mid, 0);
-            perform(slice, top, sh);
-            const Sum s = total();
-            if (s.n >= k || s.lo >= reach) {
-                lo = mid;
-            } else {
-                hi = mid;
-            }
+        if (inside > kList && hi - lo > 1) {
             command(kSumAbove, hi, hi, 0);
             perform(slice, top, sh);
-            const uint32_t above = total().n;
+            uint32_t above = total().n;
+            const double reach = by_mass ? top_p * total().hi : INFINITY;
             command(kSumAbove, lo, lo, 0);
             perform(slice, top, sh);
-            inside = total().n - above;
+            uint32_t upto = total().n;
+            while (upto - above > kList && hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                command(kSumAbove, mid, mid, 0);
+                perform(slice, top, sh);
+                const Sum s = total();
+                if (s.n >= k || s.lo >= reach)
+                    lo = mid, upto = s.n;
+                else
+                    hi = mid, above = s.n;
+            }
+            inside = upto - above;
         }
         const bool ties = inside > kList;  // (of one key)
         __syncthreads();
@@ -1044,6 +1091,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         command(ties ? kGatherTies : kGather, hi, lo, 0);
         perform(slice, top, sh);
         const Sum above = total();
+        const double reach = by_mass ? top_p * above.hi : INFINITY;  // (Z in 64 bits)
         if (ties) {
             tie_key = lo;
             const double w = weigh(value_of(lo));
@@ -1079,14 +1127,14 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             cut = keep ? list[order[keep - 1]] : (uint64_t)hi << 32;
             kept = above.n + keep;
             // (the chunks' maxima have served: each tile's share of the list, in units whose sums know no order)
-            uint64_t* share = reinterpret_cast<uint64_t*>(chunk_max);
-            for (uint32_t t = threadIdx.x; t < tiles; t += kThreads) share[t] = 0;
+            uint32_t* share = reinterpret_cast<uint32_t*>(chunk_max);
+            for (uint32_t t = threadIdx.x; t < 3 * tiles; t += kThreads) share[t] = 0;
             __syncthreads();
+#pragma unroll 4
             for (uint32_t i = threadIdx.x; i < count; i += kThreads)
-                if (list[i] >= cut)
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&share[(~(uint32_t)list[i] + row.skew) / kTile]), units_of(list[i]));
+                if (list[i] >= cut) add_units(share + 3 * ((~(uint32_t)list[i] + row.skew) / kTile), units_of(list[i]));
             __syncthreads();
-            for (uint32_t t = threadIdx.x; t < tiles; t += kThreads) tile_sum[t] += (double)share[t] * 0x1p-51;
+            for (uint32_t t = threadIdx.x; t < tiles; t += kThreads) tile_sum[t] += (double)read_units(share + 3 * t) * 0x1p-51;
         }
     }
     leave();
@@ -1113,68 +1161,47 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         sh.part[0].lo = base;
     }
     __syncthreads();
-    if (warp == 0) {
-        double before_v = sh.part[0].lo;
-        const uint32_t quota = tie_keep ? reinterpret_cast<uint32_t*>(chunk_max)[tile] : 0;
-        uint32_t seen = 0, token = kAll, final = kAll;
-        double w_token = 0.0, w_final = 0.0;
-        for (uint32_t i = 0; i < View::kLoads && token == kAll; ++i) {
-            float v[kVec];
-            double w[kVec], sum = 0.0;
-            const uint32_t j = tile * kTile + i * View::kLoad + lane * kVec;
-            row.vec(j, v);
-            uint32_t tied = 0;
+    // inside the tile, four elements a thread
+    base = sh.part[0].lo;
+    const uint32_t quota = tie_keep ? reinterpret_cast<uint32_t*>(chunk_max)[tile] : 0;
+    const uint32_t j = tile * kTile + threadIdx.x * 4;
+    float v[4];
+    row.quad(j, v);
+    uint32_t tied = 0;
 #pragma unroll
-            for (uint32_t e = 0; e < kVec; ++e) tied += tie_keep && key_of(v[e]) == tie_key;
-            uint32_t rank_before = tied;
+    for (uint32_t e = 0; e < 4; ++e) tied += tie_keep && key_of(v[e]) == tie_key;
+    uint32_t seen = 0;
+    if (tie_keep) {
+        uint32_t unused;
+        block_scan_words(tied, 0, &seen, &unused, sh);
+    }
+    double w[4];
+    s = Sum{0, 0.0, 0.0};
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const uint32_t q = __shfl_up_sync(kAll, rank_before, o);
-                if (lane >= o) rank_before += q;
-            }
-            const uint32_t chunk_ties = __shfl_sync(kAll, rank_before, 31);
-            uint32_t q = seen + rank_before - tied;
-            seen += chunk_ties;
+    for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t key = key_of(v[e]);
+        bool in = key >= kLowest && ((uint64_t)key << 32 | ~(j + e - row.skew)) >= cut;
+        if (tie_keep && key == tie_key) in = seen++ < quota;
+        w[e] = in ? weigh(v[e]) : 0.0;
+        s.lo += w[e];
+    }
+    block_scan(s, &before, sh);
+    double here = base + before.lo, w_first = 0.0, w_last = 0.0;
+    uint32_t first = kAll, end = 0;
 #pragma unroll
-            for (uint32_t e = 0; e < kVec; ++e) {
-                const uint32_t key = key_of(v[e]);
-                const uint64_t entry = (uint64_t)key << 32 | ~(j + e - row.skew);
-                bool in = key >= kLowest && entry >= cut;
-                if (tie_keep && key == tie_key) in = q++ < quota;
-                w[e] = in ? weigh(v[e]) : 0.0;
-                sum += w[e];
-            }
-            double inc = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const double d = __shfl_up_sync(kAll, inc, o);
-                if (lane >= o) inc += d;
-            }
-            double here = before_v + (inc - sum);
-            uint32_t mine = kAll, mine_last = 0;
-            double w_mine = 0.0, w_last = 0.0;
-#pragma unroll
-            for (uint32_t e = 0; e < kVec; ++e) {
-                here += w[e];
-                if (w[e] > 0.0) {
-                    mine_last = j + e - row.skew + 1, w_last = w[e];
-                    if (mine == kAll && here > target && before_v < INFINITY) mine = j + e - row.skew, w_mine = w[e];
-                }
-            }
-            const uint32_t first = __reduce_min_sync(kAll, mine);
-            if (first != kAll) {
-                const uint32_t who = __ffs(__ballot_sync(kAll, mine == first)) - 1;
-                token = first, w_token = __shfl_sync(kAll, w_mine, who);
-            }
-            const uint32_t end = __reduce_max_sync(kAll, mine_last);
-            if (end) {
-                const uint32_t who = __ffs(__ballot_sync(kAll, mine_last == end)) - 1;
-                final = end - 1, w_final = __shfl_sync(kAll, w_last, who);
-            }
-            before_v += __shfl_sync(kAll, inc, 31);
+    for (uint32_t e = 0; e < 4; ++e) {
+        here += w[e];
+        if (w[e] > 0.0) {
+            if (first == kAll && here > target && base < INFINITY) first = j + e - row.skew, w_first = w[e];
+            end = j + e - row.skew + 1, w_last = w[e];
         }
-        if (token == kAll) token = final, w_token = w_final;
-        if (lane == 0) finish(LRS_OK, token, w_token / mass, kept);
+    }
+    uint32_t token = block_min(first, sh);
+    if (token == kAll) {  // (two orders of a sum: the last one with weight)
+        token = ~block_min(~end, sh) - 1;
+        if (end == token + 1) finish(LRS_OK, token, w_last / mass, kept);
+    } else if (first == token) {
+        finish(LRS_OK, token, w_first / mass, kept);
     }
 }
 
@@ -1183,7 +1210,7 @@ constexpr int kMaxDevices = 64;
 template <typename T>
 size_t shared_bytes(uint32_t n) {
     const uint32_t tiles = (n + 15 + kTile - 1) / kTile;
-    return kList * 8 + kChunks * 4 + kSlots * 8 + (tiles + 1) / 2 * 2 * 8 + (size_t)tiles * kPer * 4;
+    return kList * 8 + kChunks * 4 + kSlots * 12 + (tiles + 1) / 2 * 2 * 8 + (size_t)tiles * kPer * 4;
 }
 
 template <typename T>
