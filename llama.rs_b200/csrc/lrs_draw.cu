@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         return;  // (every CTA of the cluster)
     }
     const uint32_t n = g.n;
-    View row;
+    RowView<T> row;
     {
         const T* x = reinterpret_cast<const T*>(g.logits) + r * g.ld;
         row.skew = (uint32_t)((uintptr_t)x % 16 / sizeof(T));
