@@ -97,8 +97,8 @@ struct Bound {
     bool bounded;
     __device__ __forceinline__ float distance(float x) const { return (0.5f * top - 0.5f * x) * scale; }
     __device__ __forceinline__ bool operator()(float x) const {
-        const float f = distance(x);
-        return x >= least && (!bounded || f < edge0 - 1.0f || (f < edge0 && (f - (edge0 - 1.0f)) * 256.0f < edge1));
+        const float f = distance(x);  // (without branches: many are tested side by side)
+        return (x >= least) & (!bounded | (f < edge0 - 1.0f) | ((f < edge0) & ((f - (edge0 - 1.0f)) * 256.0f < edge1)));
     }
 };
 
@@ -319,18 +319,22 @@ struct RowView {
             for (uint32_t i = 0; i < kVec; ++i) v[i] = j + i >= skew && j + i < end ? to_float<T>(base[j + i]) : -INFINITY;
         }
     }
-    // four elements from position j (a multiple of four)
+    // four elements from position j (a multiple of four), all within the row
+    __device__ __forceinline__ void whole_quad(uint32_t j, float (&v)[4]) const {
+        if constexpr (sizeof(T) == 4) {
+            unpack(__ldg(reinterpret_cast<const uint4*>(base + j)), v, base);
+        } else {
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(base + j));
+            float x[8];
+            unpack(make_uint4(q.x, q.y, 0, 0), x, base);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = x[i];
+        }
+    }
+    // the same anywhere; -inf outside the row
     __device__ __forceinline__ void quad(uint32_t j, float (&v)[4]) const {
         if (j >= skew && j + 4 <= end) {
-            if constexpr (sizeof(T) == 4) {
-                unpack(__ldg(reinterpret_cast<const uint4*>(base + j)), v, base);
-            } else {
-                const uint2 q = __ldg(reinterpret_cast<const uint2*>(base + j));
-                float x[8];
-                unpack(make_uint4(q.x, q.y, 0, 0), x, base);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = x[i];
-            }
+            whole_quad(j, v);
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) v[i] = j + i >= skew && j + i < end ? to_float<T>(base[j + i]) : -INFINITY;
@@ -417,9 +421,11 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-// Appends the elements of a lane's bit mask to the first CTA's list: one addition to its count a warp.
-template <typename T, int N, typename Index>
-__device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const float (&v)[N], uint32_t mask, Index index) {
+// Appends the elements of the lanes' bit masks to the first CTA's list: one addition to its count a warp,
+// and as many turns as the fullest lane has elements (they are read again: registers have no index).
+template <typename T, typename At>
+__device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const RowView<T>& row, uint32_t mask, At position) {
+    if (!__any_sync(kAll, mask != 0)) return;
     const uint32_t lane = threadIdx.x % 32, mine = __popc(mask);
     uint32_t inc = mine;
 #pragma unroll
@@ -427,17 +433,12 @@ __device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const fl
         const uint32_t q = __shfl_up_sync(kAll, inc, o);
         if (lane >= o) inc += q;
     }
-    const uint32_t all = __shfl_sync(kAll, inc, 31);
-    if (all == 0) return;
     uint32_t at = 0;
-    if (lane == 31) at = atomicAdd(count, all);
+    if (lane == 31) at = atomicAdd(count, inc);
     at = __shfl_sync(kAll, at, 31) + inc - mine;
-    if (mask == 0) return;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (!(mask >> i & 1)) continue;
-        if (at < kList) list[at] = (uint64_t)key_of(v[i]) << 32 | ~index(i);
-        ++at;
+    for (; mask; mask &= mask - 1, ++at) {
+        const uint32_t j = position(__ffs(mask) - 1);
+        if (at < kList) list[at] = (uint64_t)key_of(to_float<T>(row.base[j])) << 32 | ~(j - row.skew);
     }
 }
 
@@ -450,8 +451,8 @@ struct Slice {
     uint8_t* dynamic;    // (as the kernel lays it out)
     double* first_sum;
     float* first_max;
-    __device__ __forceinline__ uint32_t index(uint32_t t, int i) const {  // of element i of a lane's 32
-        return t * kTile + i / RowView<T>::kVec * RowView<T>::kLoad + threadIdx.x % 32 * RowView<T>::kVec + i % RowView<T>::kVec - row.skew;
+    __device__ __forceinline__ uint32_t position(uint32_t t, int i) const {  // of element i of a lane's 32
+        return t * kTile + i / RowView<T>::kVec * RowView<T>::kLoad + threadIdx.x % 32 * RowView<T>::kVec + i % RowView<T>::kVec;
     }
 };
 
@@ -468,12 +469,14 @@ __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
         uint32_t mask = 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) mask |= bound(v[i]) ? 1u << i : 0u;
-        append<T>(first_list, first_count, v, mask, [&](int i) { return z.index(t, i); });
+        append(first_list, first_count, z.row, mask, [&](int i) { return z.position(t, i); });
     }
 }
 
-// The upper end of a bin's weights as a power of two, 2^edge.
-__device__ __forceinline__ float bin_edge(uint32_t key, float max, float c) { return ceilf((value_of(key) - max) * c); }
+// A power of two above a bin's weights: 2^edge, by at most a factor of four (round to nearest by addition).
+__device__ __forceinline__ float bin_edge(uint32_t key, float max, float c) {
+    return (fmaxf((value_of(key) - max) * c, -1000.0f) + 12582912.0f) - 12582911.0f;
+}
 
 // Counts and masses of the keys of [lo, hi) in bins of 2^shift keys, the highest first, to the first CTA's
 // bins (clear before); returns the count and mass (64 bits) of the keys above.
@@ -489,23 +492,30 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
         __syncthreads();
     }
     const Weigh weigh{(double)max, z.c};
-    const float cf = (float)z.c, scale = (float)mass_unit(z.n);
+    const float cf = (float)z.c, scale = (float)min(mass_unit(z.n), 1u << 22);
     Sum s{0, 0.0, 0.0};
     for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
         float v[32];
         z.row.tile(t, v);
+        uint32_t above = 0;
+        // (without branches but the additions': their chains overlap)
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const uint32_t key = key_of(v[i]);
-            if (key >= hi) {
-                s.lo += weigh(v[i]), ++s.n;
-            } else if (key >= lo) {
-                const uint32_t b = (hi - 1 - key) >> shift;
-                float e;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v[i] - max) * cf - bin_edge(hi - 1 - (b << shift), max, cf)));
+            const uint32_t b = (hi - 1 - key) >> shift;
+            float e;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v[i] - max) * cf - bin_edge(hi - 1 - (b << shift), max, cf)));
+            const uint32_t w = __float_as_uint(fmaf(fminf(e, 1.0f), scale, 8388608.0f)) - 0x4B000000u;  // (below 2^23)
+            above |= key >= hi ? 1u << i : 0u;
+            if ((key >= lo) & (key < hi)) {
                 atomicAdd(&bin_n[b], 1u);
-                atomicAdd(&bin_w[b], __float2uint_rn(fminf(e, 2.0f) * scale));
+                atomicAdd(&bin_w[b], w);
             }
+        }
+        if (__any_sync(kAll, above != 0)) {
+            s.n += __popc(above);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s.lo += above >> i & 1 ? weigh(v[i]) : 0.0;
         }
     }
     if (rank) {
@@ -537,8 +547,9 @@ __device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
             const uint32_t key = key_of(v[i]);
             const double w = weigh(v[i]);
             s.hi += w;
-            if (key >= hi) above += w, ++s.n;
-            mask |= key >= lo && key < hi ? 1u << i : 0u;
+            above += key >= hi ? w : 0.0;
+            s.n += key >= hi;
+            mask |= (key >= lo) & (key < hi) ? 1u << i : 0u;
         }
         s.lo += above;
         if (op == kSumAbove) continue;
@@ -548,7 +559,7 @@ __device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
             const uint32_t ties = __reduce_add_sync(kAll, __popc(mask));
             if (lane == 0) reinterpret_cast<uint32_t*>(z.first_max)[t] = ties;
         } else {
-            append<T>(first_list, first_count, v, mask, [&](int i) { return z.index(t, i); });
+            append(first_list, first_count, z.row, mask, [&](int i) { return z.position(t, i); });
         }
     }
     return s;
@@ -842,14 +853,23 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 for (uint32_t i = warp * 8; i < reaching; i += kWarps * 8) {
                     float v[32];
                     uint32_t from[8], mask = 0;
+                    bool whole_chunks = true;
 #pragma unroll
                     for (uint32_t q = 0; q < 8; ++q) {
-                        from[q] = i + q < reaching ? again[i + q] * kChunk + lane * 4 : row.end;
-                        row.quad(from[q], *reinterpret_cast<float(*)[4]>(&v[4 * q]));
+                        from[q] = i + q < reaching ? again[i + q] * kChunk : row.end;
+                        whole_chunks &= (from[q] >= row.skew) & (from[q] + kChunk <= row.end);
+                        from[q] += lane * 4;
+                    }
+                    if (whole_chunks) {  // (eight loads in flight)
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; ++q) row.whole_quad(from[q], *reinterpret_cast<float(*)[4]>(&v[4 * q]));
+                    } else {
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; ++q) row.quad(from[q], *reinterpret_cast<float(*)[4]>(&v[4 * q]));
                     }
 #pragma unroll
                     for (int q = 0; q < 32; ++q) mask |= bound(v[q]) ? 1u << q : 0u;
-                    append<T>(list, &sh.count, v, mask, [&](int q) { return from[q / 4] + q % 4 - row.skew; });
+                    append(list, &sh.count, row, mask, [&](int q) { return again[i + q / 4] * kChunk + lane * 4 + q % 4; });
                 }
             }
             __syncthreads();
@@ -1031,14 +1051,14 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             // element, and the 32-bit power), Z within its own
             constexpr uint32_t kEach = kBins / kThreads;
             const float cf = (float)c;
-            const double unit = 1.0 / (double)mass_unit(n);
+            const double unit = 1.0 / (double)min(mass_unit(n), 1u << 22);
             auto step = [&](uint32_t b, Sum* run) {  // adds bin b
                 const uint32_t w = bin_w[b], m = bin_n[b];
                 run->n += m;
                 if (m == 0 || !by_mass) return;
                 const uint32_t key = hi - 1 - (b << shift);
                 const float up = bin_edge(key, top, cf);
-                if (up < -900.0f) return;  // (weighs nothing)
+                if (up < -900.0f) return;  // (weighs nothing: powers of two end there)
                 const double s = unit * __hiloint2double((1023 + (int)up) << 20, 0);
                 const double err = 0x1p-20 * (3.0 - (double)up);
                 run->lo += fmax(0.0, ((double)w - m) * s * (1.0 - err)), run->hi += ((double)w + m) * s * (1.0 + err);
