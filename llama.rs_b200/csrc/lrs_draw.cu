@@ -237,56 +237,14 @@ __device__ __forceinline__ uint64_t read_units(const uint32_t* sum) {
 }
 
 constexpr uint32_t kSlots = 512;  // of the bins below
-constexpr uint32_t kOwn = kList / kThreads;
 
-// order[i] = place in the list of its i-th largest entry: entries are dealt into bins by their value
-// between the list's ends, and ranked within their bin by comparison.  Lists that crowd a bin (long runs
-// of equal values) are sorted in place.
-__device__ __noinline__ void rank_list(uint64_t* list, uint16_t* order, uint32_t* slots, uint32_t count, Shared& sh) {
-    uint32_t* ends = slots + kSlots;
-    uint32_t least = kAll, most = 0;
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
-        const uint32_t key = (uint32_t)(list[i] >> 32);
-        least = min(least, key), most = max(most, key);
-    }
-    const float low = value_of(block_min(least, sh)), top = value_of(~block_min(~most, sh));
-    const float scale = low < top ? fminf((float)kSlots * 0.999f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f;
-    auto slot = [&](uint64_t entry) {
-        return min((uint32_t)((0.5f * top - 0.5f * value_of((uint32_t)(entry >> 32))) * scale), kSlots - 1);
-    };
-    for (uint32_t i = threadIdx.x; i < kSlots; i += kThreads) slots[i] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) atomicAdd(&slots[slot(list[i])], 1u);
-    __syncthreads();
-    const uint32_t a = slots[2 * threadIdx.x], b = slots[2 * threadIdx.x + 1];
-    uint32_t before, unused;
-    block_scan_words(a + b, 0, &before, &unused, sh);
-    ends[2 * threadIdx.x] = before, ends[2 * threadIdx.x + 1] = before + a;
-    if (__syncthreads_or(a > kSlots || b > kSlots)) {
-        sort(list, count);
-        for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[i] = (uint16_t)i;
-        __syncthreads();
-        return;
-    }
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[atomicAdd(&ends[slot(list[i])], 1u)] = (uint16_t)i;
-    __syncthreads();
-    uint16_t place[kOwn];
-#pragma unroll
-    for (uint32_t q = 0; q < kOwn; ++q) {
-        const uint32_t i = threadIdx.x + q * kThreads;
-        if (i >= count) break;
-        const uint64_t entry = list[i];
-        const uint32_t s = slot(entry), end = ends[s];
-        uint32_t rank = end - slots[s];
-        for (uint32_t j = rank; j < end; ++j) rank += list[order[j]] > entry;
-        place[q] = (uint16_t)rank;
-    }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t q = 0; q < kOwn; ++q)
-        if (threadIdx.x + q * kThreads < count) order[place[q]] = (uint16_t)(threadIdx.x + q * kThreads);
-    __syncthreads();
-}
+// Where the kept elements of a list end: `entry` is the last one kept (in descending order), `keep` how
+// many are, `sure` whether both ends of Z's error give the same.
+struct Cut {
+    uint64_t entry;
+    uint32_t keep;
+    bool sure;
+};
 
 struct Args {
     const void* logits;
@@ -518,11 +476,16 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
             for (int i = 0; i < 32; ++i) s.lo += above >> i & 1 ? weigh(v[i]) : 0.0;
         }
     }
-    if (rank) {
-        __syncthreads();
-        uint32_t* first_bin = cluster.map_shared_rank(bin_n, 0);
-        for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads)
-            if (bin_n[i]) atomicAdd(&first_bin[i], bin_n[i]);
+    const uint32_t ctas = cluster.num_blocks();
+    if (ctas > 1) {  // each CTA adds up a part of the bins over all of them, into the first one's
+        cluster.sync();
+        const uint32_t each = 2 * kBins / ctas;  // (a power of two)
+        for (uint32_t i = rank * each + threadIdx.x; i < (rank + 1) * each; i += kThreads) {
+            uint32_t sum = 0;
+#pragma unroll 4
+            for (uint32_t q = 0; q < ctas; ++q) sum += cluster.map_shared_rank(bin_n, q)[i];
+            cluster.map_shared_rank(bin_n, 0)[i] = sum;
+        }
     }
     return s;
 }
@@ -582,6 +545,122 @@ __device__ void perform(const Slice<T>& z, float max, Shared& sh) {
         __syncthreads();
 }
 
+// A weight in whole numbers of 2^-51: their sums do not depend on an order.
+__device__ __forceinline__ uint64_t units(const Weigh& weigh, uint64_t entry) {
+    return __double2ull_rn(weigh(value_of((uint32_t)(entry >> 32))) * 0x1p51);
+}
+// What of `reach` is left above `base`, in the same units.
+__device__ __forceinline__ uint64_t units_left(double reach, double base) {
+    return __double2ull_ru(fmin(fmax(reach - base, 0.0) * 0x1p51, 0x1p63));
+}
+
+// The cut of a list (zeros: dropped entries) below base_n kept elements of mass base: the entries are dealt
+// into slots by their value between the list's ends, the slots' counts and masses summed from the top,
+// and the entries of the slot that fills k or `reach` compared with one another.  A slot that too many
+// share (long runs of nearly equal values) has the list sorted instead.
+__device__ __noinline__ Cut find_cut(uint64_t* list, uint32_t* slots, uint32_t* members, uint32_t count, uint32_t base_n,
+                                     double base, uint32_t k, bool by_mass, double reach_lo, double reach_hi,
+                                     const Weigh weigh, Shared& sh) {
+    uint32_t least = kAll, most = 0, mine = 0;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t key = (uint32_t)(list[i] >> 32);
+        if (key) least = min(least, key), most = max(most, key), ++mine;
+    }
+    const uint32_t least_key = block_min(least, sh);
+    const float low = value_of(least_key), top = value_of(~block_min(~most, sh));
+    const uint32_t real = block_scan(Sum{mine, 0.0, 0.0}, nullptr, sh).n;
+    if (real == 0) return Cut{~0ull, 0, true};
+    auto all = [&] {  // every entry is kept: the lowest of them
+        uint32_t last = kAll;
+        for (uint32_t i = threadIdx.x; i < count; i += kThreads)
+            if ((uint32_t)(list[i] >> 32) == least_key) last = min(last, (uint32_t)list[i]);
+        return Cut{(uint64_t)least_key << 32 | block_min(last, sh), real, true};
+    };
+    if (!by_mass && k - base_n >= real) return all();
+    const float scale = low < top ? fminf((float)kSlots * 0.999f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f;
+    auto slot_of = [&](uint64_t entry) {
+        return min((uint32_t)((0.5f * top - 0.5f * value_of((uint32_t)(entry >> 32))) * scale), kSlots - 1);
+    };
+    const uint64_t goal_lo = by_mass ? units_left(reach_lo, base) : ~0ull, goal_hi = by_mass ? units_left(reach_hi, base) : ~0ull;
+    const uint32_t goal_n = k - base_n;
+    uint32_t* slot_n = slots;            // counts, and masses of three words
+    uint32_t* slot_w = slots + kSlots;
+    for (uint32_t i = threadIdx.x; i < 4 * kSlots; i += kThreads) slots[i] = 0;
+    if (threadIdx.x == 0) sh.chunks = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint64_t e = list[i];
+        if (!e) continue;
+        const uint32_t at = slot_of(e);
+        atomicAdd(&slot_n[at], 1u);
+        if (by_mass) add_units(slot_w + 3 * at, units(weigh, e));
+    }
+    __syncthreads();
+    const uint32_t one = 2 * threadIdx.x, two = one + 1;
+    uint32_t before_n, unused;
+    uint64_t before = 0, w1 = 0, w2 = 0;
+    block_scan_words(slot_n[one] + slot_n[two], 0, &before_n, &unused, sh);
+    if (by_mass) {
+        w1 = read_units(slot_w + 3 * one), w2 = read_units(slot_w + 3 * two);
+        block_scan_long(w1 + w2, &before, sh);
+    }
+    const uint32_t n1 = before_n + slot_n[one], n2 = n1 + slot_n[two];
+    auto hit = [&](uint64_t goal) {
+        const uint32_t at = n1 >= goal_n || before + w1 >= goal ? one : n2 >= goal_n || before + w1 + w2 >= goal ? two : kAll;
+        return block_min(at, sh);
+    };
+    const uint32_t at = hit(goal_lo), at_hi = by_mass ? hit(goal_hi) : at;
+    if (at != at_hi) return Cut{0, 0, false};
+    if (at == kAll) return all();
+    if (at == one || at == two) sh.count = at == one ? before_n : n1, sh.cut = at == one ? before : before + w1;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        if (!list[i] || slot_of(list[i]) != at) continue;
+        const uint32_t m = atomicAdd(&sh.chunks, 1u);
+        if (m < kThreads) members[m] = i;
+    }
+    __syncthreads();
+    const uint32_t in = sh.chunks, above_n = sh.count;
+    const uint64_t above = sh.cut;
+    __syncthreads();
+    if (in <= kThreads) {
+        uint64_t* mass = reinterpret_cast<uint64_t*>(slots);  // (the slots have served)
+        const uint64_t e = threadIdx.x < in ? list[members[threadIdx.x]] : 0;
+        if (by_mass && e) mass[threadIdx.x] = units(weigh, e);
+        __syncthreads();
+        uint32_t rank = above_n;
+        uint64_t over = above;
+        if (e)
+            for (uint32_t j = 0; j < in; ++j) {
+                const bool more = list[members[j]] > e;
+                rank += more;
+                if (by_mass) over += more ? mass[j] : 0;
+            }
+        const bool keep = e && rank < goal_n && over < goal_lo, keep_hi = e && rank < goal_n && over < goal_hi;
+        if (__syncthreads_or(keep != keep_hi)) return Cut{0, 0, false};
+        const uint32_t kept = __syncthreads_count(keep);
+        // (none: there was nothing left to fill; else the last one kept is one of the slot that fills it)
+        if (kept == 0) return Cut{~0ull, 0, true};
+        if (keep && rank + 1 == above_n + kept) sh.cut = e;
+        __syncthreads();
+        return Cut{sh.cut, above_n + kept, true};
+    }
+    sort(list, count);
+    const uint32_t per = (real + kThreads - 1) / kThreads;
+    const uint32_t i0 = min(real, threadIdx.x * per), i1 = min(real, i0 + per);
+    uint64_t sum = 0, run;
+    if (by_mass)
+        for (uint32_t i = i0; i < i1; ++i) sum += units(weigh, list[i]);
+    block_scan_long(sum, &run, sh);
+    uint32_t a = 0, b = 0;
+    for (uint32_t i = i0; i < i1; ++i) {
+        a += i < goal_n && run < goal_lo, b += i < goal_n && run < goal_hi;
+        if (by_mass) run += units(weigh, list[i]);
+    }
+    const uint32_t keep = block_scan(Sum{a, 0.0, 0.0}, nullptr, sh).n, keep_hi = block_scan(Sum{b, 0.0, 0.0}, nullptr, sh).n;
+    return Cut{keep ? list[keep - 1] : ~0ull, keep, keep == keep_hi};
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     extern __shared__ __align__(16) uint8_t dynamic[];
@@ -624,9 +703,8 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     uint32_t* bin_n = reinterpret_cast<uint32_t*>(dynamic);                // kBins counts and
     uint32_t* bin_w = bin_n + kBins;                                       // kBins masses
     uint32_t* again = reinterpret_cast<uint32_t*>(list + kList);           // kChunks chunk numbers
-    uint16_t* order = reinterpret_cast<uint16_t*>(again);                  // (later) the list's order
-    uint32_t* slots = again + kChunks;                                     // 3 kSlots words
-    double* tile_sum = reinterpret_cast<double*>(slots + 3 * kSlots);      // a tile's
+    uint32_t* slots = again + kChunks;                                     // 4 kSlots words
+    double* tile_sum = reinterpret_cast<double*>(slots + 4 * kSlots);      // a tile's
     float* chunk_max = reinterpret_cast<float*>(tile_sum + (tiles + 1) / 2 * 2);
     double* first_sum = cluster.map_shared_rank(tile_sum, 0);
     float* first_max = cluster.map_shared_rank(chunk_max, 0);
@@ -752,29 +830,16 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     const double top_p = (double)p.top_p;
     double reach_lo = by_mass ? top_p * z * (1.0 - kApprox) : INFINITY, reach_hi = by_mass ? top_p * z * (1.0 + kApprox) : INFINITY;
 
-    // Ordered candidates (below `base` kept elements): how many of them are kept.
-    auto cut_list = [&](uint32_t count, const Sum& base, double reach_a, double reach_b, uint32_t* at_b) {
-        const uint32_t per = (count + kThreads - 1) / kThreads;
-        const uint32_t i0 = min(count, threadIdx.x * per), i1 = min(count, i0 + per);
-        Sum s{0, 0.0, 0.0}, before;
+    auto units_of = [&](uint64_t entry) { return units(weigh, entry); };
+    // Entries lighter than min_p leave the list.
+    auto drop_light = [&](uint32_t count) {
+        if (p.min_p > 0.0f) {
 #pragma unroll 4
-        for (uint32_t i = i0; i < i1; ++i) s.lo += weigh(value_of((uint32_t)(list[order[i]] >> 32)));
-        block_scan(s, &before, sh);
-        double run = base.lo + before.lo;
-        uint32_t a = 0, b = 0;
-#pragma unroll 4
-        for (uint32_t i = i0; i < i1; ++i) {
-            const double w = weigh(value_of((uint32_t)(list[order[i]] >> 32)));
-            const bool in = base.n + i < k && w >= (double)p.min_p;
-            a += in && run < reach_a;
-            b += in && run < reach_b;
-            run += w;
+            for (uint32_t i = threadIdx.x; i < count; i += kThreads)
+                if (!(weigh(value_of((uint32_t)(list[i] >> 32))) >= (double)p.min_p)) list[i] = 0;
         }
-        const Sum both = block_scan(Sum{a | b << 16, 0.0, 0.0}, nullptr, sh);  // (at most 4096 each)
-        *at_b = both.n >> 16;
-        return both.n & 0xFFFFu;
+        __syncthreads();
     };
-    auto units_of = [&](uint64_t entry) { return __double2ull_rn(weigh(value_of((uint32_t)(entry >> 32))) * 0x1p51); };
 
     if (!whole) {
         // ---- 2. few survivors ----
@@ -939,27 +1004,13 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 return leave();
             }
             if (count <= kList) {
-                uint64_t cut = 0;  // the last entry kept
-                uint32_t keep = count;
-                if (by_mass || k < count) {
-                    rank_list(list, order, slots, count, sh);
-                    uint32_t other;
-                    keep = cut_list(count, Sum{0, 0.0, 0.0}, reach_lo, reach_hi, &other);
-                    if (keep != other) {  // Z's error decides
-                        z = row_mass();
-                        keep = cut_list(count, Sum{0, 0.0, 0.0}, top_p * z, top_p * z, &other);
-                    }
-                    cut = list[order[keep - 1]];
-                } else if (p.min_p > 0.0f) {
-                    uint32_t mine = 0;
-                    for (uint32_t i = threadIdx.x; i < count; i += kThreads)
-                        if (weigh(value_of((uint32_t)(list[i] >> 32))) >= (double)p.min_p)
-                            ++mine;
-                        else
-                            list[i] = 0;
-                    keep = block_scan(Sum{mine, 0.0, 0.0}, nullptr, sh).n;
-                    cut = 1;
+                drop_light(count);
+                Cut kept = find_cut(list, slots, again, count, 0, 0.0, k, by_mass, reach_lo, reach_hi, weigh, sh);
+                if (!kept.sure) {  // Z's error decides
+                    z = row_mass();
+                    kept = find_cut(list, slots, again, count, 0, 0.0, k, by_mass, top_p * z, top_p * z, weigh, sh);
                 }
+                const uint64_t cut = kept.entry;
                 // The token: masses (whole numbers of 2^-51: their sums know no order) by ranges of indices,
                 // the range that the target falls in again by parts where it is crowded, then its entries.
                 uint32_t* range = slots;  // three words each
@@ -1013,7 +1064,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 uint32_t token = block_min(weighs && (double)upto > target ? index : kAll, sh);
                 if (token == kAll) token = ~block_min(weighs ? ~index : kAll, sh);
                 if (entry && index == token)
-                    finish(LRS_OK, token, weigh(value_of((uint32_t)(entry >> 32))) * 0x1p51 / (double)total, keep);
+                    finish(LRS_OK, token, weigh(value_of((uint32_t)(entry >> 32))) * 0x1p51 / (double)total, kept.keep);
                 return leave();
             }
         }
@@ -1048,31 +1099,39 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             perform(slice, top, sh);
             base = total();
             // where the cut may lie: counts are exact, masses within their rounding (half a unit an
-            // element, and the 32-bit power), Z within its own
+            // element, and the 32-bit power), Z within its own; masses here in 2^-40
             constexpr uint32_t kEach = kBins / kThreads;
             const float cf = (float)c;
-            const double unit = 1.0 / (double)min(mass_unit(n), 1u << 22);
-            auto step = [&](uint32_t b, Sum* run) {  // adds bin b
+            const int unit = 31 - __clz(min(mass_unit(n), 1u << 22));  // a bin's masses are in 2^(edge - unit)
+            auto fixed = [](double mass) { return __double2ull_rd(fmin(fmax(mass, 0.0) * 0x1p40, 0x1p63)); };
+            auto bin = [&](uint32_t b, uint64_t* lo_mass, uint64_t* hi_mass) {
                 const uint32_t w = bin_w[b], m = bin_n[b];
-                run->n += m;
-                if (m == 0 || !by_mass) return;
-                const uint32_t key = hi - 1 - (b << shift);
-                const float up = bin_edge(key, top, cf);
-                if (up < -900.0f) return;  // (weighs nothing: powers of two end there)
-                const double s = unit * __hiloint2double((1023 + (int)up) << 20, 0);
-                const double err = 0x1p-20 * (3.0 - (double)up);
-                run->lo += fmax(0.0, ((double)w - m) * s * (1.0 - err)), run->hi += ((double)w + m) * s * (1.0 + err);
+                if (m == 0 || !by_mass) return m;
+                const int up = (int)bin_edge(hi - 1 - (b << shift), top, cf), left = up + 40 - unit;
+                if (left <= -32) {  // (weighs nothing)
+                    *hi_mass += 1;
+                    return m;
+                }
+                auto at = [&](uint64_t v) { return left >= 0 ? v << left : v >> -left; };
+                const uint64_t l = at(w > m ? w - m : 0), h = at((uint64_t)w + m) + 1;
+                const uint64_t err = (uint64_t)(3 - up);  // in 2^-20 of the mass
+                *lo_mass += l - min(l, (l >> 20) * err + err), *hi_mass += h + (h >> 20) * err + err;
+                return m;
             };
-            Sum s{0, 0.0, 0.0}, before;
-            for (uint32_t i = 0; i < kEach; ++i) step(threadIdx.x * kEach + i, &s);
-            block_scan(s, &before, sh);
-            Sum run{base.n + before.n, base.lo + before.lo, base.lo + before.hi};
-            uint32_t a = kBins - 1, z1 = kBins - 1;
+            uint32_t own_n = 0, before_n, unused;
+            uint64_t own_lo = 0, own_hi = 0, run_lo, run_hi;
+            for (uint32_t i = 0; i < kEach; ++i) own_n += bin(threadIdx.x * kEach + i, &own_lo, &own_hi);
+            block_scan_words(own_n, 0, &before_n, &unused, sh);
+            block_scan_long(own_lo, &run_lo, sh);
+            block_scan_long(own_hi, &run_hi, sh);
+            run_lo += fixed(base.lo), run_hi += fixed(base.lo) + 1;
+            const uint64_t goal_lo = by_mass ? fixed(reach_lo) : ~0ull, goal_hi = by_mass ? fixed(reach_hi) + 1 : ~0ull;
+            uint32_t run_n = base.n + before_n, a = kBins - 1, z1 = kBins - 1;
             for (uint32_t i = 0; i < kEach; ++i) {
                 const uint32_t b = threadIdx.x * kEach + i;
-                step(b, &run);
-                if ((run.n >= k || run.hi >= reach_lo) && b < a) a = b;
-                if ((run.n >= k || run.lo >= reach_hi) && b < z1) z1 = b;
+                run_n += bin(b, &run_lo, &run_hi);
+                if ((run_n >= k || run_hi >= goal_lo) && b < a) a = b;
+                if ((run_n >= k || run_lo >= goal_hi) && b < z1) z1 = b;
             }
             a = block_min(a, sh), z1 = block_min(z1, sh);
             const uint32_t last = (range - 1) >> shift;
@@ -1141,11 +1200,10 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             }
         } else {
             const uint32_t count = min(sh.count, kList);
-            rank_list(list, order, slots, count, sh);
-            uint32_t other;
-            const uint32_t keep = cut_list(count, above, reach, reach, &other);
-            cut = keep ? list[order[keep - 1]] : (uint64_t)hi << 32;
-            kept = above.n + keep;
+            drop_light(count);
+            const Cut end = find_cut(list, slots, again, count, above.n, above.lo, k, by_mass, reach, reach, weigh, sh);
+            cut = end.keep ? end.entry : (uint64_t)hi << 32;
+            kept = above.n + end.keep;
             // (the chunks' maxima have served: each tile's share of the list, in units whose sums know no order)
             uint32_t* share = reinterpret_cast<uint32_t*>(chunk_max);
             for (uint32_t t = threadIdx.x; t < 3 * tiles; t += kThreads) share[t] = 0;
@@ -1230,7 +1288,7 @@ constexpr int kMaxDevices = 64;
 template <typename T>
 size_t shared_bytes(uint32_t n) {
     const uint32_t tiles = (n + 15 + kTile - 1) / kTile;
-    return kList * 8 + kChunks * 4 + kSlots * 12 + (tiles + 1) / 2 * 2 * 8 + (size_t)tiles * kPer * 4;
+    return kList * 8 + kChunks * 4 + kSlots * 16 + (tiles + 1) / 2 * 2 * 8 + (size_t)tiles * kPer * 4;
 }
 
 template <typename T>
