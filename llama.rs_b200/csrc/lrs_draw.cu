@@ -239,11 +239,11 @@ __device__ __forceinline__ uint64_t read_units(const uint32_t* sum) {
 constexpr uint32_t kSlots = 512;  // of the bins below
 
 // Where the kept elements of a list end: `entry` is the last one kept (in descending order), `keep` how
-// many are, `sure` whether both ends of Z's error give the same.
+// many are, `sure` whether both ends of Z's error give the same, `filled` whether k or the mass was, or entries had been dropped.
 struct Cut {
     uint64_t entry;
     uint32_t keep;
-    bool sure;
+    bool sure, filled;
 };
 
 struct Args {
@@ -431,6 +431,10 @@ __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
     }
 }
 
+// Where bin b is kept: threads that read kBins / kThreads neighbouring bins each meet all banks.
+constexpr uint32_t kBinWords = kBins + kThreads;
+__device__ __forceinline__ uint32_t bin_place(uint32_t b) { return b + b / (kBins / kThreads); }
+
 // A power of two above a bin's weights: 2^edge, by at most a factor of four (round to nearest by addition).
 __device__ __forceinline__ float bin_edge(uint32_t key, float max, float c) {
     return (fmaxf((value_of(key) - max) * c, -1000.0f) + 12582912.0f) - 12582911.0f;
@@ -443,10 +447,10 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t hi = sh.order[1], lo = sh.order[2], shift = sh.order[3];
     uint32_t* bin_n = reinterpret_cast<uint32_t*>(z.dynamic);
-    uint32_t* bin_w = bin_n + kBins;
+    uint32_t* bin_w = bin_n + kBinWords;
     const uint32_t rank = cluster.block_rank();
     if (rank) {
-        for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads) bin_n[i] = 0;
+        for (uint32_t i = threadIdx.x; i < 2 * kBinWords; i += kThreads) bin_n[i] = 0;
         __syncthreads();
     }
     const Weigh weigh{(double)max, z.c};
@@ -466,8 +470,8 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
             const uint32_t w = __float_as_uint(fmaf(fminf(e, 1.0f), scale, 8388608.0f)) - 0x4B000000u;  // (below 2^23)
             above |= key >= hi ? 1u << i : 0u;
             if ((key >= lo) & (key < hi)) {
-                atomicAdd(&bin_n[b], 1u);
-                atomicAdd(&bin_w[b], w);
+                atomicAdd(&bin_n[bin_place(b)], 1u);
+                atomicAdd(&bin_w[bin_place(b)], w);
             }
         }
         if (__any_sync(kAll, above != 0)) {
@@ -479,7 +483,7 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
     const uint32_t ctas = cluster.num_blocks();
     if (ctas > 1) {  // each CTA adds up a part of the bins over all of them, into the first one's
         cluster.sync();
-        const uint32_t each = 2 * kBins / ctas;  // (a power of two)
+        const uint32_t each = 2 * kBinWords / ctas;  // (a whole number for 1, 2, 4, 8, 16)
         for (uint32_t i = rank * each + threadIdx.x; i < (rank + 1) * each; i += kThreads) {
             uint32_t sum = 0;
 #pragma unroll 4
@@ -569,12 +573,12 @@ __device__ __noinline__ Cut find_cut(uint64_t* list, uint32_t* slots, uint32_t* 
     const uint32_t least_key = block_min(least, sh);
     const float low = value_of(least_key), top = value_of(~block_min(~most, sh));
     const uint32_t real = block_scan(Sum{mine, 0.0, 0.0}, nullptr, sh).n;
-    if (real == 0) return Cut{~0ull, 0, true};
+    if (real == 0) return Cut{~0ull, 0, true, false};
     auto all = [&] {  // every entry is kept: the lowest of them
         uint32_t last = kAll;
         for (uint32_t i = threadIdx.x; i < count; i += kThreads)
             if ((uint32_t)(list[i] >> 32) == least_key) last = min(last, (uint32_t)list[i]);
-        return Cut{(uint64_t)least_key << 32 | block_min(last, sh), real, true};
+        return Cut{(uint64_t)least_key << 32 | block_min(last, sh), real, true, k - base_n <= real || real < count};
     };
     if (!by_mass && k - base_n >= real) return all();
     const float scale = low < top ? fminf((float)kSlots * 0.999f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f;
@@ -611,7 +615,7 @@ __device__ __noinline__ Cut find_cut(uint64_t* list, uint32_t* slots, uint32_t* 
         return block_min(at, sh);
     };
     const uint32_t at = hit(goal_lo), at_hi = by_mass ? hit(goal_hi) : at;
-    if (at != at_hi) return Cut{0, 0, false};
+    if (at != at_hi) return Cut{0, 0, false, false};
     if (at == kAll) return all();
     if (at == one || at == two) sh.count = at == one ? before_n : n1, sh.cut = at == one ? before : before + w1;
     for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
@@ -637,13 +641,13 @@ __device__ __noinline__ Cut find_cut(uint64_t* list, uint32_t* slots, uint32_t* 
                 if (by_mass) over += more ? mass[j] : 0;
             }
         const bool keep = e && rank < goal_n && over < goal_lo, keep_hi = e && rank < goal_n && over < goal_hi;
-        if (__syncthreads_or(keep != keep_hi)) return Cut{0, 0, false};
+        if (__syncthreads_or(keep != keep_hi)) return Cut{0, 0, false, false};
         const uint32_t kept = __syncthreads_count(keep);
         // (none: there was nothing left to fill; else the last one kept is one of the slot that fills it)
-        if (kept == 0) return Cut{~0ull, 0, true};
+        if (kept == 0) return Cut{~0ull, 0, true, true};
         if (keep && rank + 1 == above_n + kept) sh.cut = e;
         __syncthreads();
-        return Cut{sh.cut, above_n + kept, true};
+        return Cut{sh.cut, above_n + kept, true, true};
     }
     sort(list, count);
     const uint32_t per = (real + kThreads - 1) / kThreads;
@@ -658,7 +662,7 @@ __device__ __noinline__ Cut find_cut(uint64_t* list, uint32_t* slots, uint32_t* 
         if (by_mass) run += units(weigh, list[i]);
     }
     const uint32_t keep = block_scan(Sum{a, 0.0, 0.0}, nullptr, sh).n, keep_hi = block_scan(Sum{b, 0.0, 0.0}, nullptr, sh).n;
-    return Cut{keep ? list[keep - 1] : ~0ull, keep, keep == keep_hi};
+    return Cut{keep ? list[keep - 1] : ~0ull, keep, keep == keep_hi, true};
 }
 
 template <typename T>
@@ -700,8 +704,9 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     const uint32_t each = (tiles + ctas - 1) / ctas, t0 = min(tiles, rank * each), t1 = min(tiles, t0 + each);
 
     uint64_t* list = reinterpret_cast<uint64_t*>(dynamic);                 // kList entries, or
-    uint32_t* bin_n = reinterpret_cast<uint32_t*>(dynamic);                // kBins counts and
-    uint32_t* bin_w = bin_n + kBins;                                       // kBins masses
+    uint32_t* bin_n = reinterpret_cast<uint32_t*>(dynamic);                // kBinWords counts and
+    uint32_t* bin_w = bin_n + kBinWords;                                   // masses (into `again`)
+    static_assert(2 * kBinWords * 4 <= kList * 8 + kChunks * 4, "the bins fit the lists' memory");
     uint32_t* again = reinterpret_cast<uint32_t*>(list + kList);           // kChunks chunk numbers
     uint32_t* slots = again + kChunks;                                     // 4 kSlots words
     double* tile_sum = reinterpret_cast<double*>(slots + 4 * kSlots);      // a tile's
@@ -858,6 +863,13 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         const uint32_t unit = min(mass_unit(chunks), 1u << 24);
         const uint64_t mass_goal = by_mass ? __double2ull_ru(fmin(reach_hi * unit, 0x1p40)) : ~0ull;
         Bound bound{top, low < top ? fminf(255.9f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f, least, 0.0f, 1e30f, true};  // (halves: no overflow)
+        // Where they do not fill either, a bound at 4.5 % of the maxima from below leaves about 3.1 elements a
+        // chunk of 128 above it (3,700 at n = 151,936), whatever the values if they come in no order: a list that may
+        // do, and shows it if it does.  It is tried where k is that small, or the mass above the bound seems to
+        // be enough: if a share 1 - i / N of the chunks has nothing above x, -ln(1 - i / N) elements a chunk lie
+        // there, so that the i-th largest maximum stands for N / (N - i) elements.
+        const uint32_t most = (uint32_t)(n / kChunk * 0.955f);
+        bool guess = false;
         uint32_t reaching = 0;
         for (int round = 0; round < 2; ++round) {
             few_n[threadIdx.x] = 0, few_w[threadIdx.x] = 0;
@@ -883,8 +895,15 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             uint32_t before_n, before_w;
             block_scan_words(few_n[bin], few_w[bin], &before_n, &before_w, sh);
             const uint32_t upto = before_n + few_n[bin];
-            const bool fills = upto >= k || (uint64_t)before_w + few_w[bin] >= mass_goal;
-            const uint32_t at = block_min(fills ? bin : kAll, sh);
+            const bool fills = guess ? upto >= most : upto >= k || (uint64_t)before_w + few_w[bin] >= mass_goal;
+            uint32_t at = block_min(fills ? bin : kAll, sh);
+            if (at == kAll && n > kList && (by_mass || k < n)) {
+                const uint32_t edge = block_min(upto >= most ? bin : kAll, sh);
+                Sum held{0, 0.0, 0.0};
+                if (bin <= edge) held.lo = few_w[bin] * ((double)chunks / (chunks - min(before_n + few_n[bin] / 2, chunks - 1)));
+                guess = k <= kList * 7 / 8 || (by_mass && block_scan(held, nullptr, sh).lo >= 0.9 * (double)mass_goal);
+                if (guess) at = edge;
+            }
             if (at == kAll) {  // not even all of them: every element from `least` up
                 bound.bounded = false;
                 break;
@@ -896,9 +915,10 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 bound.edge0 = (float)(at + 1);
             else
                 bound.edge1 = (float)(at + 1);
-            if (reaching <= (k < chunks ? k + 32 : 64)) break;
+            if (reaching <= (guess ? most + 16 : k < chunks ? k + 32 : 64)) break;
             __syncthreads();
         }
+        guess &= !bound(least);  // (what passes `least` is all there is)
         __syncthreads();
         if (threadIdx.x == 0) sh.count = 0, sh.chunks = 0, sh.bound = bound;
         __syncthreads();
@@ -949,7 +969,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 }
                 return block_scan(s, nullptr, sh).lo;
             };
-            if (count <= kFew) {
+            if (count <= kFew && !guess) {
                 // Every candidate's rank and the mass before it by comparison with all, the comparisons of
                 // one shared by `lanes` neighbours; masses are whole numbers of 2^-51, so that their sums do
                 // not depend on the list's order.
@@ -1003,13 +1023,18 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 if (real && part == 0 && index == token) finish(LRS_OK, token, w * 0x1p51 / (double)total, kept);
                 return leave();
             }
-            if (count <= kList) {
-                drop_light(count);
-                Cut kept = find_cut(list, slots, again, count, 0, 0.0, k, by_mass, reach_lo, reach_hi, weigh, sh);
-                if (!kept.sure) {  // Z's error decides
-                    z = row_mass();
-                    kept = find_cut(list, slots, again, count, 0, 0.0, k, by_mass, top_p * z, top_p * z, weigh, sh);
+            while (count <= kList) {
+                Cut kept{1, 0, true, true};
+                const bool light = p.min_p > 0.0f && !by_mass && k >= n;  // min_p alone: tested below
+                if (!light) {
+                    drop_light(count);
+                    kept = find_cut(list, slots, again, count, 0, 0.0, k, by_mass, reach_lo, reach_hi, weigh, sh);
+                    if (!kept.sure) {  // Z's error decides
+                        z = row_mass();
+                        kept = find_cut(list, slots, again, count, 0, 0.0, k, by_mass, top_p * z, top_p * z, weigh, sh);
+                    }
                 }
+                if (guess && !kept.filled) break;
                 const uint64_t cut = kept.entry;
                 // The token: masses (whole numbers of 2^-51: their sums know no order) by ranges of indices,
                 // the range that the target falls in again by parts where it is crowded, then its entries.
@@ -1017,6 +1042,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 uint32_t first = 0, width = (n + kSlots - 1) / kSlots;  // indices from `first`, `width` a range
                 uint64_t below = 0, total = 0;
                 double target = 0.0;
+                uint32_t mine = 0;
                 for (int round = 0; round < 2; ++round) {
                     __syncthreads();
                     for (uint32_t i = threadIdx.x; i < 3 * kSlots; i += kThreads) range[i] = 0;
@@ -1026,7 +1052,14 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                     for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
                         const uint64_t e = list[i];
                         const uint32_t slot = (~(uint32_t)e - first) / width;  // (before `first`: out of range too)
-                        if (e >= cut && slot < kSlots) add_units(range + 3 * slot, units_of(e));
+                        if (e < cut || slot >= kSlots) continue;
+                        const double w = weigh(value_of((uint32_t)(e >> 32)));
+                        if (light && !(w >= (double)p.min_p)) {
+                            list[i] = 0;
+                            continue;
+                        }
+                        mine += round == 0;
+                        add_units(range + 3 * slot, __double2ull_rn(w * 0x1p51));
                     }
                     __syncthreads();
                     const uint64_t a = read_units(range + 6 * threadIdx.x), b = read_units(range + 6 * threadIdx.x + 3);
@@ -1052,6 +1085,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                     width = (width + kSlots - 1) / kSlots;  // (at most 2^22 / 512 / 512 = 16 indices then)
                 }
                 const uint32_t members = sh.count;
+                if (light) kept.keep = block_scan(Sum{mine, 0.0, 0.0}, nullptr, sh).n;
                 const uint64_t entry = threadIdx.x < members ? list[again[threadIdx.x]] : 0;
                 const uint32_t index = ~(uint32_t)entry;
                 uint64_t upto = below;
@@ -1094,7 +1128,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             const uint32_t bits = 32 - __clz(range - 1 | 1);
             const uint32_t shift = bits > 12 ? bits - 12 : 0;
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < 2 * kBins; i += kThreads) bin_n[i] = 0;
+            for (uint32_t i = threadIdx.x; i < 2 * kBinWords; i += kThreads) bin_n[i] = 0;
             command(kHistogram, hi, lo, shift);
             perform(slice, top, sh);
             base = total();
@@ -1105,7 +1139,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             const int unit = 31 - __clz(min(mass_unit(n), 1u << 22));  // a bin's masses are in 2^(edge - unit)
             auto fixed = [](double mass) { return __double2ull_rd(fmin(fmax(mass, 0.0) * 0x1p40, 0x1p63)); };
             auto bin = [&](uint32_t b, uint64_t* lo_mass, uint64_t* hi_mass) {
-                const uint32_t w = bin_w[b], m = bin_n[b];
+                const uint32_t w = bin_w[bin_place(b)], m = bin_n[bin_place(b)];
                 if (m == 0 || !by_mass) return m;
                 const int up = (int)bin_edge(hi - 1 - (b << shift), top, cf), left = up + 40 - unit;
                 if (left <= -32) {  // (weighs nothing)
@@ -1137,7 +1171,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             const uint32_t last = (range - 1) >> shift;
             a = min(a, last), z1 = min(z1, last);
             Sum in{0, 0.0, 0.0};
-            for (uint32_t b = a + threadIdx.x; b <= z1; b += kThreads) in.n += bin_n[b];
+            for (uint32_t b = a + threadIdx.x; b <= z1; b += kThreads) in.n += bin_n[bin_place(b)];
             inside = block_scan(in, nullptr, sh).n;
             const uint32_t from = hi;
             hi = from - (a << shift);

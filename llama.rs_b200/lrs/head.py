@@ -13,71 +13,66 @@ cudaStream_t handle of that device) where one is given.
 """
 from __future__ import annotations
 
-from .sampler import LRS_E_INVALID, SamplerError, _check, _Launch, dtype_code, lib
+from .sampler import LRS_E_INVALID, SamplerError, dtype_code, launch, lib
 
 BLOCK = 128
 
 
-def _matrix(t, what: str):
-    """A 2-d CUDA tensor of contiguous rows: its leading dimension (rows of one have none)."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise SamplerError(LRS_E_INVALID, f"{what}: a 2-d tensor with contiguous rows is needed")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _codes(t, rows: int, k: int, what: str):
-    if t.element_size() != 1 or tuple(t.shape) != (rows, k):
-        raise SamplerError(LRS_E_INVALID, f"{what}: codes are 8-bit tensors of {rows} x {k}")
-    return _matrix(t, what)
-
-
-def _scales(t, a: int, b: int, what: str):
-    if dtype_code(t) != 0 or tuple(t.shape) != (a, b):
-        raise SamplerError(LRS_E_INVALID, f"{what}: scales are a float32 tensor of {a} x {b}")
-    return _matrix(t, what)
+def _matrix(t, rows: int, cols: int, size: int, what: str) -> int:
+    """The leading dimension of a rows x cols tensor of contiguous rows and `size` bytes an element (0: any);
+    rows of one have none."""
+    if t.shape != (rows, cols) or (size and t.element_size() != size):
+        raise SamplerError(LRS_E_INVALID, f"{what}: a tensor of {rows} x {cols} is needed, of {size or 'any'} bytes an element")
+    step, inner = t.stride()
+    if inner != 1 and cols > 1:
+        raise SamplerError(LRS_E_INVALID, f"{what}: contiguous rows are needed")
+    return step if rows > 1 else cols
 
 
 def _blocks(k: int) -> int:
     return (k + BLOCK - 1) // BLOCK
 
 
+def _two(t, what: str):
+    if t.dim() != 2:
+        raise SamplerError(LRS_E_INVALID, f"{what}: a 2-d tensor is needed")
+    return t.shape
+
+
+def _quantize(call, x, codes, scales, a: int, b: int, stream) -> None:
+    rows, k = x.shape
+    launch(call, stream,
+           (x.data_ptr(), dtype_code(x), rows, k, _matrix(x, rows, k, 0, "x"), codes.data_ptr(),
+            _matrix(codes, rows, k, 1, "codes"), scales.data_ptr(), _matrix(scales, a, b, 4, "scales")),
+           x, codes, scales)
+
+
 def quantize_rows(x, codes, scales, stream=None) -> None:
     """x (rows, k) float32 / bfloat16 / float16 -> codes (rows, k) e4m3 (float8_e4m3fn or uint8) and
     scales (ceil(k / 128), rows) float32, one per row and 128 columns.  For lrs_fp8_logits let the
     codes start on 16-byte boundaries (see `empty_codes`)."""
-    rows, k = x.shape
-    ld, ldq, lds = _matrix(x, "x"), _codes(codes, rows, k, "codes"), _scales(scales, _blocks(k), rows, "scales")
-    with _Launch(stream, x, codes, scales) as s:
-        _check(lib().lrs_quantize_rows(x.data_ptr(), dtype_code(x), rows, k, ld, codes.data_ptr(), ldq,
-                                       scales.data_ptr(), max(lds, rows), s))
+    rows, k = _two(x, "x")
+    _quantize(lib().lrs_quantize_rows, x, codes, scales, _blocks(k), rows, stream)
 
 
 def quantize_blocks(x, codes, scales, stream=None) -> None:
     """x (rows, k) -> codes (rows, k) e4m3 and scales (ceil(rows / 128), ceil(k / 128)) float32, one per
     128 x 128 block."""
-    rows, k = x.shape
-    kb = _blocks(k)
-    ld, ldq, lds = _matrix(x, "x"), _codes(codes, rows, k, "codes"), _scales(scales, _blocks(rows), kb, "scales")
-    with _Launch(stream, x, codes, scales) as s:
-        _check(lib().lrs_quantize_blocks(x.data_ptr(), dtype_code(x), rows, k, ld, codes.data_ptr(), ldq,
-                                         scales.data_ptr(), max(lds, kb), s))
+    rows, k = _two(x, "x")
+    _quantize(lib().lrs_quantize_blocks, x, codes, scales, _blocks(rows), _blocks(k), stream)
 
 
 def fp8_logits(a, a_scales, w, w_scales, out, stream=None) -> None:
     """out (rows, n) = a (rows, k) times w (n, k) transposed, both e4m3 codes with the scales of
     quantize_rows and quantize_blocks; out is float32, bfloat16 or float16."""
-    rows, k = a.shape
-    n = w.shape[0]
-    lda, ldw = _codes(a, rows, k, "a"), _codes(w, n, k, "w")
-    kb = _blocks(k)
-    ldas, ldws = _scales(a_scales, kb, rows, "a_scales"), _scales(w_scales, _blocks(n), kb, "w_scales")
-    if tuple(out.shape) != (rows, n):
-        raise SamplerError(LRS_E_INVALID, f"out: a tensor of {rows} x {n} is needed")
-    ldo = _matrix(out, "out")
-    with _Launch(stream, a, a_scales, w, w_scales, out) as s:
-        _check(lib().lrs_fp8_logits(a.data_ptr(), lda, a_scales.data_ptr(), max(ldas, rows), w.data_ptr(), ldw,
-                                    w_scales.data_ptr(), max(ldws, kb), rows, n, k, out.data_ptr(), dtype_code(out),
-                                    ldo, s))
+    rows, k = _two(a, "a")
+    n, kb = w.shape[0], _blocks(k)
+    launch(lib().lrs_fp8_logits, stream,
+           (a.data_ptr(), _matrix(a, rows, k, 1, "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, 4, "a_scales"),
+            w.data_ptr(), _matrix(w, n, k, 1, "w"), w_scales.data_ptr(),
+            _matrix(w_scales, _blocks(n), kb, 4, "w_scales"), rows, n, k, out.data_ptr(), dtype_code(out),
+            _matrix(out, rows, n, 0, "out")),
+           a, a_scales, w, w_scales, out)
 
 
 def empty_codes(rows: int, k: int, device):
@@ -103,7 +98,7 @@ class LmHead:
         the hidden states come from torch's allocator, so calls on several streams and captured
         calls do not share them."""
         import torch
-        rows, k = hidden.shape
+        rows, k = _two(hidden, "hidden")
         if k != self.k:
             raise SamplerError(LRS_E_INVALID, f"hidden: {k} columns, the head has {self.k}")
         if out is None:

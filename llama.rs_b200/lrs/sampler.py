@@ -164,32 +164,39 @@ def dtype_code(t) -> int:
     return code
 
 
-class _Launch:
-    """The device and stream of a call without a context: checks that the tensors (None: absent) lie
-    on one GPU, makes it the current device while the call is enqueued, and gives the stream's
-    handle (torch's current stream there unless `stream` is given)."""
-    __slots__ = ("stream", "device", "back")
+_raw_stream = None
 
-    def __init__(self, stream, *tensors):
-        d = tensors[0].get_device()
-        if d < 0:
-            raise SamplerError(LRS_E_INVALID, "CUDA tensors are needed")
-        for t in tensors:
-            if t is not None and t.get_device() != d:
-                raise SamplerError(LRS_E_INVALID, "the tensors lie on different devices")
-        self.stream, self.device = stream, d
 
-    def __enter__(self):
+def current_stream(device: int) -> int:
+    """The handle of torch's current stream on a device."""
+    global _raw_stream
+    if _raw_stream is None:
         import torch
-        self.back = torch.cuda.current_device()
-        if self.back != self.device:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream if self.stream is None else self.stream
+        # (a tenth of the time of building a Stream object, where this torch has it)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
-    def __exit__(self, *exc):
-        if self.back != self.device:
-            import torch
-            torch.cuda.set_device(self.back)
+
+def launch(call, stream, args, *tensors) -> None:
+    """Enqueues call(*args, stream handle) on the GPU of the tensors (None: absent), which have to lie on one: on
+    torch's current stream there unless `stream` gives a handle.  Leaves the current device as it was."""
+    import torch
+    device = tensors[0].get_device()
+    if device < 0:
+        raise SamplerError(LRS_E_INVALID, "CUDA tensors are needed")
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise SamplerError(LRS_E_INVALID, "the tensors lie on different devices")
+    if stream is None:
+        stream = current_stream(device)
+    if torch.cuda.current_device() == device:
+        code = call(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            code = call(*args, stream)
+    if code != LRS_OK:
+        _check(code)
 
 
 class Sampler:
@@ -299,26 +306,27 @@ class BatchSampler:
         probs float32.  The definition of the kept set and of the draw is the header's.  Async; no
         working memory and no context, so calls may overlap and be captured."""
         rows = tokens.numel() if rows is None else rows
-        if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        if logits.dim() != 2:
+            raise SamplerError(LRS_E_INVALID, "logits: a 2-d tensor is needed")
+        have, width = logits.shape
+        step, inner = logits.stride()
+        if inner != 1 and width > 1:
             raise SamplerError(LRS_E_INVALID, "logits: a 2-d tensor with contiguous rows is needed")
-        n = logits.shape[1] if n is None else n
+        n = width if n is None else n
         if ld is None:
-            ld = logits.stride(0) if logits.shape[0] > 1 else n if rows <= 1 else 0
-        have = logits.shape[0] if ld else rows
-        if rows > have or n > logits.shape[1] or params.numel() * params.element_size() < 16 * rows:
+            ld = step if have > 1 else n if rows <= 1 else 0
+        if (rows > have and ld) or n > width or params.numel() * params.element_size() < 16 * rows:
             raise SamplerError(LRS_E_INVALID, f"draw_device: the logits or the parameters hold fewer than {rows} rows of {n}")
-        for t in (params, uniform, tokens, probs, kept, status):
-            if t is not None and not t.is_contiguous():
-                raise SamplerError(LRS_E_INVALID, "draw_device: a buffer of a value a row is not contiguous")
         for t in (uniform, tokens, probs, kept, status):
-            if t is not None and (t.numel() < rows or t.element_size() != 4):
-                raise SamplerError(LRS_E_INVALID, f"draw_device: a buffer holds fewer than {rows} 32-bit values")
-        with _Launch(stream, logits, params, uniform, tokens, probs, kept, status) as s:
-            _check(lib().lrs_draw_device(logits.data_ptr(), dtype_code(logits), rows, n, ld, params.data_ptr(),
-                                         uniform.data_ptr(), tokens.data_ptr(),
-                                         None if probs is None else probs.data_ptr(),
-                                         None if kept is None else kept.data_ptr(),
-                                         None if status is None else status.data_ptr(), s))
+            if t is not None and (t.numel() < rows or t.element_size() != 4 or not t.is_contiguous()):
+                raise SamplerError(LRS_E_INVALID, f"draw_device: a buffer is not {rows} 32-bit values in a row")
+        if not params.is_contiguous():
+            raise SamplerError(LRS_E_INVALID, "draw_device: the parameters are not contiguous")
+        launch(lib().lrs_draw_device, stream,
+               (logits.data_ptr(), dtype_code(logits), rows, n, ld, params.data_ptr(), uniform.data_ptr(),
+                tokens.data_ptr(), None if probs is None else probs.data_ptr(),
+                None if kept is None else kept.data_ptr(), None if status is None else status.data_ptr()),
+               logits, params, uniform, tokens, probs, kept, status)
 
     @staticmethod
     def draw_hidden(head, hidden, params, uniform, tokens, probs=None, kept=None, status=None, dtype=None):
