@@ -22,6 +22,7 @@
 #include <cooperative_groups.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "lrs_ops.cuh"
 
@@ -60,24 +61,37 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 }
 
 // 2^y for y <= about 0: the fraction's power by a polynomial (2^f - 1) / f of degree 8 through
-// Chebyshev nodes on [-1/2, 1/2], 3.7e-14 off at most and exact at 0; 0 below 2^-1000.
+// Chebyshev nodes on [-1/2, 1/2], 3.7e-14 off at most and exact at 0; 0 below 2^-1000.  N side by side: a
+// chain of 14 operations of the 64-bit pipe is long, and the compiler does not weave unrolled ones.
+template <int N>
+__device__ __forceinline__ void power2(const double (&y)[N], double (&r)[N]) {
+    constexpr double kMagic = 0x1.8p52;
+    constexpr double kTerms[9] = {0x1.63d136366db24p-20, 0x1.ffcb9515a8016p-17, 0x1.4308ac85aa947p-13,
+                                  0x1.5d87fe86fe88ep-10, 0x1.3b2ab7181b755p-7, 0x1.c6b08d7047e52p-5,
+                                  0x1.ebfbdff823cedp-3, 0x1.62e42fefa39efp-1, 1.0};
+    double t[N], f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = y[i] + kMagic;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = t[i] - kMagic;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = y[i] - f[i], r[i] = 0x1.b63880a30e9ffp-24;
+#pragma unroll
+    for (int k = 0; k < 9; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = fma(r[i], f[i], kTerms[k]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool gone = (uint32_t)__double2hiint(y[i]) > 0xC08F4000u;  // y < -1000, -inf included
+        const double p = __hiloint2double(__double2hiint(r[i]) + (__double2loint(t[i]) << 20), __double2loint(r[i]));
+        r[i] = gone ? 0.0 : p;
+    }
+}
 __device__ __forceinline__ double power2(double y) {
-    const double magic = 0x1.8p52;
-    const double t = y + magic, f = y - (t - magic);
-    double p = 0x1.b63880a30e9ffp-24;
-    p = fma(p, f, 0x1.63d136366db24p-20);
-    p = fma(p, f, 0x1.ffcb9515a8016p-17);
-    p = fma(p, f, 0x1.4308ac85aa947p-13);
-    p = fma(p, f, 0x1.5d87fe86fe88ep-10);
-    p = fma(p, f, 0x1.3b2ab7181b755p-7);
-    p = fma(p, f, 0x1.c6b08d7047e52p-5);
-    p = fma(p, f, 0x1.ebfbdff823cedp-3);
-    p = fma(p, f, 0x1.62e42fefa39efp-1);
-    p = fma(p, f, 1.0);
-    const uint32_t top = (uint32_t)__double2hiint(y);
-    const bool gone = top > 0xC08F4000u;  // y < -1000, -inf included
-    const double r = __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
-    return gone ? 0.0 : r;
+    const double in[1] = {y};
+    double out[1];
+    power2(in, out);
+    return out[0];
 }
 
 struct Sum {
@@ -265,17 +279,19 @@ struct RowView {
     const T* base;
     uint32_t skew, end;  // elements are base[skew .. end)
 
-    // V consecutive elements from position j (a multiple of V); -inf outside the row
-    __device__ __forceinline__ void vec(uint32_t j, float* v) const {
-        if (j >= skew && j + kVec <= end) {
-            float x[kVec];
-            unpack(__ldg(reinterpret_cast<const uint4*>(base + j)), x, base);
+    // -inf, kVec (or two words of it: half) times
+    static __device__ __forceinline__ uint32_t nothing() {
+        return sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+    }
+    __device__ __forceinline__ bool holds(uint32_t j, uint32_t count) const { return (j >= skew) & (j + count <= end); }
+    // count elements from position j some of which are outside the row: -inf there
+    template <uint32_t COUNT>
+    __device__ __forceinline__ void piece(uint32_t j, float* v) const {
+        T x[COUNT];
 #pragma unroll
-            for (uint32_t i = 0; i < kVec; ++i) v[i] = x[i];
-        } else {
+        for (uint32_t i = 0; i < COUNT; ++i) x[i] = base[min(max(j + i, skew), end - 1)];  // (in flight together)
 #pragma unroll
-            for (uint32_t i = 0; i < kVec; ++i) v[i] = j + i >= skew && j + i < end ? to_float<T>(base[j + i]) : -INFINITY;
-        }
+        for (uint32_t i = 0; i < COUNT; ++i) v[i] = holds(j + i, 1) ? to_float<T>(x[i]) : -INFINITY;
     }
     // four elements from position j (a multiple of four), all within the row
     __device__ __forceinline__ void whole_quad(uint32_t j, float (&v)[4]) const {
@@ -289,31 +305,40 @@ struct RowView {
             for (int i = 0; i < 4; ++i) v[i] = x[i];
         }
     }
-    // the same anywhere; -inf outside the row
     __device__ __forceinline__ void quad(uint32_t j, float (&v)[4]) const {
-        if (j >= skew && j + 4 <= end) {
+        if (holds(j, 4))
             whole_quad(j, v);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) v[i] = j + i >= skew && j + i < end ? to_float<T>(base[j + i]) : -INFINITY;
-        }
+        else
+            piece<4>(j, v);
     }
+    // A lane's 32 elements of a tile, -inf outside the row.  The loads go out together, those of the row's
+    // ends too: taken one after the other there, a tile took 8 us and not 1.
     __device__ __forceinline__ void tile(uint32_t t, float (&v)[32]) const {
         const uint32_t j = t * kTile + threadIdx.x % 32 * kVec;
-        if (t * kTile >= skew && t * kTile + kTile <= end) {
-            uint4 r[kLoads];
+        uint4 r[kLoads];
+        const bool inner = holds(t * kTile, kTile);
+        if (inner) {
 #pragma unroll
             for (uint32_t c = 0; c < kLoads; ++c) r[c] = __ldg(reinterpret_cast<const uint4*>(base + j + c * kLoad));
-#pragma unroll
-            for (uint32_t c = 0; c < kLoads; ++c) {
-                float x[kVec];
-                unpack(r[c], x, base);
-#pragma unroll
-                for (uint32_t i = 0; i < kVec; ++i) v[c * kVec + i] = x[i];
-            }
         } else {
 #pragma unroll
-            for (uint32_t c = 0; c < kLoads; ++c) vec(j + c * kLoad, v + c * kVec);
+            for (uint32_t c = 0; c < kLoads; ++c) {
+                r[c] = make_uint4(nothing(), nothing(), nothing(), nothing());
+                if (holds(j + c * kLoad, kVec)) r[c] = __ldg(reinterpret_cast<const uint4*>(base + j + c * kLoad));
+            }
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < kLoads; ++c) {
+            float x[kVec];
+            unpack(r[c], x, base);
+#pragma unroll
+            for (uint32_t i = 0; i < kVec; ++i) v[c * kVec + i] = x[i];
+        }
+        if (inner) return;
+#pragma unroll
+        for (uint32_t c = 0; c < kLoads; ++c) {  // (a vector at either end)
+            const uint32_t at = j + c * kLoad;
+            if (!holds(at, kVec) && at < end && at + kVec > skew) piece<kVec>(at, v + c * kVec);
         }
     }
     // the maxima of the tile's chunks: lane i < kPer gets chunk i's; a NaN stays
@@ -338,10 +363,33 @@ struct RowView {
     }
 };
 
+constexpr int kWeave = 4;
+
 // Weights relative to a maximum.
 struct Weigh {
     double max, c;
     __device__ __forceinline__ double operator()(float x) const { return power2(((double)x - max) * c); }
+    template <int N>
+    __device__ __forceinline__ void many(const float* x, double (&w)[N]) const {
+        double y[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = ((double)x[i] - max) * c;
+        power2(y, w);
+    }
+    // the sum of a lane's 32
+    __device__ __forceinline__ double sum(const float (&v)[32]) const {
+        double s[kWeave] = {};
+#pragma unroll
+        for (int i = 0; i < 32; i += kWeave) {
+            double w[kWeave];
+            many(v + i, w);
+#pragma unroll
+            for (int j = 0; j < kWeave; ++j) s[j] += w[j];
+        }
+#pragma unroll
+        for (int j = 1; j < kWeave; ++j) s[0] += s[j];
+        return s[0];
+    }
 };
 
 // 32-bit tile sums: 2^(x c) = 2^f 2^k, k the nearest integer to x c and f the rest, exact to 2^-26
@@ -379,10 +427,9 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-// Appends the elements of the lanes' bit masks to the first CTA's list: one addition to its count a warp,
-// and as many turns as the fullest lane has elements (they are read again: registers have no index).
-template <typename T, typename At>
-__device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const RowView<T>& row, uint32_t mask, At position) {
+// Appends the elements of the lanes' bit masks to the first CTA's list: one addition to its count a warp.
+template <int N, typename At>
+__device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const float (&v)[N], uint32_t mask, At index) {
     if (!__any_sync(kAll, mask != 0)) return;
     const uint32_t lane = threadIdx.x % 32, mine = __popc(mask);
     uint32_t inc = mine;
@@ -394,9 +441,11 @@ __device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const Ro
     uint32_t at = 0;
     if (lane == 31) at = atomicAdd(count, inc);
     at = __shfl_sync(kAll, at, 31) + inc - mine;
-    for (; mask; mask &= mask - 1, ++at) {
-        const uint32_t j = position(__ffs(mask) - 1);
-        if (at < kList) list[at] = (uint64_t)key_of(to_float<T>(row.base[j])) << 32 | ~(j - row.skew);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool hit = mask >> i & 1;
+        if (hit & (at < kList)) list[at] = (uint64_t)key_of(v[i]) << 32 | ~index(i);
+        at += hit;
     }
 }
 
@@ -409,31 +458,51 @@ struct Slice {
     uint8_t* dynamic;    // (as the kernel lays it out)
     double* first_sum;
     float* first_max;
-    __device__ __forceinline__ uint32_t position(uint32_t t, int i) const {  // of element i of a lane's 32
-        return t * kTile + i / RowView<T>::kVec * RowView<T>::kLoad + threadIdx.x % 32 * RowView<T>::kVec + i % RowView<T>::kVec;
+    __device__ __forceinline__ uint32_t index(uint32_t t, int i) const {  // of element i of a lane's 32
+        return t * kTile + i / RowView<T>::kVec * RowView<T>::kLoad + threadIdx.x % 32 * RowView<T>::kVec + i % RowView<T>::kVec - row.skew;
     }
 };
 
-// Candidates: the elements that pass the bound, to the first CTA's list.
+// Candidates: the elements that pass the bound, to the first CTA's list, from the chunks that it has listed
+// (shared out over all warps).  Four chunks at a time: their loads are in flight together.
 template <typename T>
 __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
+    constexpr uint32_t kGroup = 4;
     cg::cluster_group cluster = cg::this_cluster();
     uint64_t* first_list = cluster.map_shared_rank(reinterpret_cast<uint64_t*>(z.dynamic), 0);
+    const uint32_t* again = reinterpret_cast<const uint32_t*>(first_list + kList);
     uint32_t* first_count = cluster.map_shared_rank(&sh.count, 0);
     const Bound bound = sh.bound;
-    for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
-        float v[32];
-        z.row.tile(t, v);
-        uint32_t mask = 0;
+    const uint32_t reaching = sh.order[1], lane = threadIdx.x % 32;
+    const uint32_t warps = cluster.num_blocks() * kWarps, me = cluster.block_rank() * kWarps + threadIdx.x / 32;
+    for (uint32_t i = me * kGroup; i < reaching; i += warps * kGroup) {
+        float v[4 * kGroup];
+        uint32_t from[kGroup], mask = 0;
+        bool whole_chunks = true;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mask |= bound(v[i]) ? 1u << i : 0u;
-        append(first_list, first_count, z.row, mask, [&](int i) { return z.position(t, i); });
+        for (uint32_t q = 0; q < kGroup; ++q) {
+            from[q] = again[min(i + q, reaching - 1)] * kChunk;  // (past the end: the last again, not listed)
+            whole_chunks &= z.row.holds(from[q], kChunk);
+            from[q] += lane * 4;
+        }
+        if (whole_chunks) {
+#pragma unroll
+            for (uint32_t q = 0; q < kGroup; ++q) z.row.whole_quad(from[q], *reinterpret_cast<float(*)[4]>(&v[4 * q]));
+        } else {
+#pragma unroll
+            for (uint32_t q = 0; q < kGroup; ++q) z.row.template piece<4>(from[q], v + 4 * q);
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < 4 * kGroup; ++q) mask |= bound(v[q]) & (i + q / 4 < reaching) ? 1u << q : 0u;
+        append(first_list, first_count, v, mask, [&](int q) { return from[q / 4] + q % 4 - z.row.skew; });
     }
 }
 
-// Where bin b is kept: threads that read kBins / kThreads neighbouring bins each meet all banks.
+// Where bin b is kept: a word is left free after every kEachBin bins, a thread's share of them, so that
+// threads that read their shares meet all banks.
+constexpr uint32_t kEachBin = kBins / kThreads;
 constexpr uint32_t kBinWords = kBins + kThreads;
-__device__ __forceinline__ uint32_t bin_place(uint32_t b) { return b + b / (kBins / kThreads); }
+__device__ __forceinline__ uint32_t bin_place(uint32_t b) { return b + b / kEachBin; }
 
 // A power of two above a bin's weights: 2^edge, by at most a factor of four (round to nearest by addition).
 __device__ __forceinline__ float bin_edge(uint32_t key, float max, float c) {
@@ -460,7 +529,7 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
         float v[32];
         z.row.tile(t, v);
         uint32_t above = 0;
-        // (without branches but the additions': their chains overlap)
+        // (without a branch, so that the chains overlap: what is outside goes to words that no bin uses)
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const uint32_t key = key_of(v[i]);
@@ -469,15 +538,19 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v[i] - max) * cf - bin_edge(hi - 1 - (b << shift), max, cf)));
             const uint32_t w = __float_as_uint(fmaf(fminf(e, 1.0f), scale, 8388608.0f)) - 0x4B000000u;  // (below 2^23)
             above |= key >= hi ? 1u << i : 0u;
-            if ((key >= lo) & (key < hi)) {
-                atomicAdd(&bin_n[bin_place(b)], 1u);
-                atomicAdd(&bin_w[bin_place(b)], w);
-            }
+            const uint32_t place = (key >= lo) & (key < hi) ? bin_place(b) : threadIdx.x % 32 * (kEachBin + 1) + kEachBin;
+            atomicAdd(&bin_n[place], 1u);
+            atomicAdd(&bin_w[place], w);
         }
         if (__any_sync(kAll, above != 0)) {
             s.n += __popc(above);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s.lo += above >> i & 1 ? weigh(v[i]) : 0.0;
+            for (int i = 0; i < 32; i += kWeave) {
+                double w[kWeave];
+                weigh.many(v + i, w);
+#pragma unroll
+                for (int j = 0; j < kWeave; ++j) s.lo += above >> (i + j) & 1 ? w[j] : 0.0;
+            }
         }
     }
     const uint32_t ctas = cluster.num_blocks();
@@ -507,18 +580,22 @@ __device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
     for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
         float v[32];
         z.row.tile(t, v);
-        double above = 0.0;
+        double above = 0.0, all = 0.0;
         uint32_t mask = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const uint32_t key = key_of(v[i]);
-            const double w = weigh(v[i]);
-            s.hi += w;
-            above += key >= hi ? w : 0.0;
-            s.n += key >= hi;
-            mask |= (key >= lo) & (key < hi) ? 1u << i : 0u;
+        for (int i = 0; i < 32; i += kWeave) {
+            double w[kWeave];
+            weigh.many(v + i, w);
+#pragma unroll
+            for (int j = 0; j < kWeave; ++j) {
+                const uint32_t key = key_of(v[i + j]);
+                all += w[j];
+                above += key >= hi ? w[j] : 0.0;
+                s.n += key >= hi;
+                mask |= (key >= lo) & (key < hi) ? 1u << (i + j) : 0u;
+            }
         }
-        s.lo += above;
+        s.lo += above, s.hi += all;
         if (op == kSumAbove) continue;
         above = warp_sum(above);
         if (lane == 0) z.first_sum[t] = above;
@@ -526,7 +603,7 @@ __device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
             const uint32_t ties = __reduce_add_sync(kAll, __popc(mask));
             if (lane == 0) reinterpret_cast<uint32_t*>(z.first_max)[t] = ties;
         } else {
-            append(first_list, first_count, z.row, mask, [&](int i) { return z.position(t, i); });
+            append(first_list, first_count, v, mask, [&](int i) { return z.index(t, i); });
         }
     }
     return s;
@@ -737,10 +814,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             if (!whole && rough.fits(tile_top)) {
                 s = warp_sum((double)rough.sum(v, tile_top));
             } else {
-                const Weigh w{(double)tile_top, c};
-#pragma unroll
-                for (int i = 0; i < 32; ++i) s += w(v[i]);
-                s = warp_sum(s);
+                s = warp_sum(Weigh{(double)tile_top, c}.sum(v));
             }
             if (whole) {
 #pragma unroll
@@ -931,31 +1005,13 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         // (without a bound the list would be the row)
         reaching = bound.bounded || p.min_p > 0.0f || n <= kList ? sh.chunks : kAll;
         if (reaching <= kChunks) {
-            if (ctas > 1 && reaching > kWarps * 8) {  // many chunks: all CTAs, each its slice
-                command(kCandidates, 0, 0, 0);
+            if (ctas > 1 && reaching > kWarps * 4) {  // many chunks: all CTAs
+                command(kCandidates, reaching, 0, 0);
                 perform(slice, top, sh);
             } else {
-                for (uint32_t i = warp * 8; i < reaching; i += kWarps * 8) {
-                    float v[32];
-                    uint32_t from[8], mask = 0;
-                    bool whole_chunks = true;
-#pragma unroll
-                    for (uint32_t q = 0; q < 8; ++q) {
-                        from[q] = i + q < reaching ? again[i + q] * kChunk : row.end;
-                        whole_chunks &= (from[q] >= row.skew) & (from[q] + kChunk <= row.end);
-                        from[q] += lane * 4;
-                    }
-                    if (whole_chunks) {  // (eight loads in flight)
-#pragma unroll
-                        for (uint32_t q = 0; q < 8; ++q) row.whole_quad(from[q], *reinterpret_cast<float(*)[4]>(&v[4 * q]));
-                    } else {
-#pragma unroll
-                        for (uint32_t q = 0; q < 8; ++q) row.quad(from[q], *reinterpret_cast<float(*)[4]>(&v[4 * q]));
-                    }
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) mask |= bound(v[q]) ? 1u << q : 0u;
-                    append(list, &sh.count, row, mask, [&](int q) { return again[i + q / 4] * kChunk + lane * 4 + q % 4; });
-                }
+                if (threadIdx.x == 0) sh.order[1] = reaching;
+                __syncthreads();
+                list_candidates(slice, sh);  // (the first warps of all are this CTA's)
             }
             __syncthreads();
             const uint32_t count = sh.count;
@@ -964,8 +1020,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 for (uint32_t t = warp; t < tiles; t += kWarps) {
                     float v[32];
                     row.tile(t, v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) s.lo += weigh(v[i]);
+                    s.lo += weigh.sum(v);
                 }
                 return block_scan(s, nullptr, sh).lo;
             };
@@ -1134,7 +1189,6 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             base = total();
             // where the cut may lie: counts are exact, masses within their rounding (half a unit an
             // element, and the 32-bit power), Z within its own; masses here in 2^-40
-            constexpr uint32_t kEach = kBins / kThreads;
             const float cf = (float)c;
             const int unit = 31 - __clz(min(mass_unit(n), 1u << 22));  // a bin's masses are in 2^(edge - unit)
             auto fixed = [](double mass) { return __double2ull_rd(fmin(fmax(mass, 0.0) * 0x1p40, 0x1p63)); };
@@ -1154,15 +1208,15 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             };
             uint32_t own_n = 0, before_n, unused;
             uint64_t own_lo = 0, own_hi = 0, run_lo, run_hi;
-            for (uint32_t i = 0; i < kEach; ++i) own_n += bin(threadIdx.x * kEach + i, &own_lo, &own_hi);
+            for (uint32_t i = 0; i < kEachBin; ++i) own_n += bin(threadIdx.x * kEachBin + i, &own_lo, &own_hi);
             block_scan_words(own_n, 0, &before_n, &unused, sh);
             block_scan_long(own_lo, &run_lo, sh);
             block_scan_long(own_hi, &run_hi, sh);
             run_lo += fixed(base.lo), run_hi += fixed(base.lo) + 1;
             const uint64_t goal_lo = by_mass ? fixed(reach_lo) : ~0ull, goal_hi = by_mass ? fixed(reach_hi) + 1 : ~0ull;
             uint32_t run_n = base.n + before_n, a = kBins - 1, z1 = kBins - 1;
-            for (uint32_t i = 0; i < kEach; ++i) {
-                const uint32_t b = threadIdx.x * kEach + i;
+            for (uint32_t i = 0; i < kEachBin; ++i) {
+                const uint32_t b = threadIdx.x * kEachBin + i;
                 run_n += bin(b, &run_lo, &run_hi);
                 if ((run_n >= k || run_hi >= goal_lo) && b < a) a = b;
                 if ((run_n >= k || run_lo >= goal_hi) && b < z1) z1 = b;
@@ -1351,11 +1405,13 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = shared_bytes<T>(g.n);
     cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ctas, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeClusterSchedulingPolicyPreference;
+    at[1].val.clusterSchedulingPolicyPreference = cudaClusterSchedulingPolicySpread;
+    cfg.attrs = at;
+    cfg.numAttrs = ctas > 1 ? 2 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g);
     return e == cudaSuccess ? LRS_OK : lrs_call_error(LRS_E_CUDA, "lrs_draw_device: launch failed: %s", cudaGetErrorString(e));
 }
