@@ -102,17 +102,15 @@ struct Sum {
 // Units of a weight of 1 in a bin's mass: the sum of n of them stays below 2^31.
 __device__ __forceinline__ uint32_t mass_unit(uint32_t n) { return 1u << (__clz((n - 1) | 1) - 2); }
 
-// A candidate's test: above the bound that the chunk maxima gave.  The distance from the maximum, in 256ths
-// of the maxima's range and in a second round in 256ths of one of those, is a monotone function of x, so
-// that a bound on it is one on x.
+// How far below the maximum the candidates reach, found from the chunk maxima: the distance in 256ths of the
+// maxima's range, and in a second round in 256ths of one of those (a monotone function of x).
 struct Bound {
-    float top, scale, least;  // nothing below `least` is kept
-    float edge0, edge1;       // candidates: distance < edge0 - 1, or within one below edge0 and the rest < edge1
-    bool bounded;
+    float top, scale;
+    float edge0, edge1;  // inside: distance < edge0 - 1, or within one below edge0 and the rest < edge1
     __device__ __forceinline__ float distance(float x) const { return (0.5f * top - 0.5f * x) * scale; }
     __device__ __forceinline__ bool operator()(float x) const {
-        const float f = distance(x);  // (without branches: many are tested side by side)
-        return (x >= least) & (!bounded | (f < edge0 - 1.0f) | ((f < edge0) & ((f - (edge0 - 1.0f)) * 256.0f < edge1)));
+        const float f = distance(x);
+        return (f < edge0 - 1.0f) | ((f < edge0) & ((f - (edge0 - 1.0f)) * 256.0f < edge1));
     }
 };
 
@@ -123,12 +121,11 @@ struct Shared {
     uint32_t word[kWarps];
     uint64_t wide[kWarps];
     uint32_t order[4];           // what the first CTA has all do next: operation, upper and lower key, shift
-    Bound bound;
     uint32_t count, chunks;      // entries of the lists
     uint64_t cut;
 };
 
-enum { kDone, kHistogram, kSumAbove, kGather, kGatherTies, kCandidates };
+enum { kDone, kLevels, kHistogram, kSumAbove, kGather, kGatherTies, kCandidates };
 
 __device__ __forceinline__ Sum add(const Sum& a, const Sum& b) { return Sum{a.n + b.n, a.lo + b.lo, a.hi + b.hi}; }
 
@@ -449,6 +446,13 @@ __device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const fl
     }
 }
 
+// The first CTA's copy of shared memory (its own for itself: the cluster's window is slower).
+template <typename P>
+__device__ __forceinline__ P* of_first(P* p) {
+    cg::cluster_group cluster = cg::this_cluster();
+    return cluster.block_rank() ? cluster.map_shared_rank(p, 0) : p;
+}
+
 // What every CTA does with its slice of the row when the first CTA says so (sh.order).
 template <typename T>
 struct Slice {
@@ -463,25 +467,24 @@ struct Slice {
     }
 };
 
-// Candidates: the elements that pass the bound, to the first CTA's list, from the chunks that it has listed
-// (shared out over all warps).  Four chunks at a time: their loads are in flight together.
+// Candidates: the elements from `least` up, to the first CTA's list, from the chunks that it has listed
+// (shared out over all warps).  Four chunks at a time, the next four on their way meanwhile.
 template <typename T>
 __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
     constexpr uint32_t kGroup = 4;
     cg::cluster_group cluster = cg::this_cluster();
-    uint64_t* first_list = cluster.map_shared_rank(reinterpret_cast<uint64_t*>(z.dynamic), 0);
+    uint64_t* first_list = of_first(reinterpret_cast<uint64_t*>(z.dynamic));
     const uint32_t* again = reinterpret_cast<const uint32_t*>(first_list + kList);
-    uint32_t* first_count = cluster.map_shared_rank(&sh.count, 0);
-    const Bound bound = sh.bound;
+    uint32_t* first_count = of_first(&sh.count);
+    const float least = value_of(sh.order[2]);
     const uint32_t reaching = sh.order[1], lane = threadIdx.x % 32;
-    const uint32_t warps = cluster.num_blocks() * kWarps, me = cluster.block_rank() * kWarps + threadIdx.x / 32;
-    for (uint32_t i = me * kGroup; i < reaching; i += warps * kGroup) {
-        float v[4 * kGroup];
-        uint32_t from[kGroup], mask = 0;
+    const uint32_t step = cluster.num_blocks() * kWarps * kGroup;
+    uint32_t i = (cluster.block_rank() * kWarps + threadIdx.x / 32) * kGroup;
+    auto load = [&](uint32_t first, uint32_t (&from)[kGroup], float (&v)[4 * kGroup]) {
         bool whole_chunks = true;
 #pragma unroll
         for (uint32_t q = 0; q < kGroup; ++q) {
-            from[q] = again[min(i + q, reaching - 1)] * kChunk;  // (past the end: the last again, not listed)
+            from[q] = again[min(first + q, reaching - 1)] * kChunk;  // (past the end: the last again, not listed)
             whole_chunks &= z.row.holds(from[q], kChunk);
             from[q] += lane * 4;
         }
@@ -492,9 +495,26 @@ __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
 #pragma unroll
             for (uint32_t q = 0; q < kGroup; ++q) z.row.template piece<4>(from[q], v + 4 * q);
         }
+    };
+    if (i >= reaching) return;
+    uint32_t from[kGroup];
+    float v[4 * kGroup];
+    load(i, from, v);
+    while (true) {
+        const uint32_t next = i + step;
+        uint32_t from_next[kGroup];
+        float v_next[4 * kGroup];
+        if (next < reaching) load(next, from_next, v_next);
+        uint32_t mask = 0;
 #pragma unroll
-        for (uint32_t q = 0; q < 4 * kGroup; ++q) mask |= bound(v[q]) & (i + q / 4 < reaching) ? 1u << q : 0u;
+        for (uint32_t q = 0; q < 4 * kGroup; ++q) mask |= (v[q] >= least) & (i + q / 4 < reaching) ? 1u << q : 0u;
         append(first_list, first_count, v, mask, [&](int q) { return from[q / 4] + q % 4 - z.row.skew; });
+        if (next >= reaching) return;
+        i = next;
+#pragma unroll
+        for (uint32_t q = 0; q < kGroup; ++q) from[q] = from_next[q];
+#pragma unroll
+        for (uint32_t q = 0; q < 4 * kGroup; ++q) v[q] = v_next[q];
     }
 }
 
@@ -503,6 +523,49 @@ __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
 constexpr uint32_t kEachBin = kBins / kThreads;
 constexpr uint32_t kBinWords = kBins + kThreads;
 __device__ __forceinline__ uint32_t bin_place(uint32_t b) { return b + b / kEachBin; }
+
+// Each CTA adds up a part of the bins over all CTAs, into the first one's.
+__device__ __forceinline__ void merge_bins(uint32_t* bins, uint32_t words) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
+    if (ctas == 1) return;
+    cluster.sync();
+    const uint32_t each = words / ctas;  // (a whole number for 1, 2, 4, 8, 16)
+    for (uint32_t i = rank * each + threadIdx.x; i < (rank + 1) * each; i += kThreads) {
+        uint32_t sum = 0;
+#pragma unroll 4
+        for (uint32_t q = 0; q < ctas; ++q) sum += cluster.map_shared_rank(bins, q)[i];
+        cluster.map_shared_rank(bins, 0)[i] = sum;
+    }
+}
+
+// A logit's level: its distance from the maximum in steps of 1 / steps, to the nearest; monotone.
+__device__ __forceinline__ uint32_t level_of(float x, float max, float steps) {
+    return __float_as_uint(fmaf(max - x, steps, 8388608.0f)) - 0x4B000000u;
+}
+
+// Counts of the levels 0 .. kBins - 1, to the first CTA's bins (clear before).  A level's weights differ by
+// so little that its mass is its count times the middle one: one addition an element.
+template <typename T>
+__device__ __noinline__ void count_levels(const Slice<T>& z, float max, Shared& sh) {
+    const float steps = __uint_as_float(sh.order[1]);
+    uint32_t* bin_n = reinterpret_cast<uint32_t*>(z.dynamic);
+    if (cg::this_cluster().block_rank()) {
+        for (uint32_t i = threadIdx.x; i < kBinWords; i += kThreads) bin_n[i] = 0;
+        __syncthreads();
+    }
+    const uint32_t spare = threadIdx.x % 32 * (kEachBin + 1) + kEachBin;
+    for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
+        float v[32];
+        z.row.tile(t, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t b = level_of(v[i], max, steps);
+            atomicAdd(&bin_n[b < kBins ? bin_place(b) : spare], 1u);
+        }
+    }
+    merge_bins(bin_n, kBinWords);
+}
 
 // A power of two above a bin's weights: 2^edge, by at most a factor of four (round to nearest by addition).
 __device__ __forceinline__ float bin_edge(uint32_t key, float max, float c) {
@@ -553,17 +616,7 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
             }
         }
     }
-    const uint32_t ctas = cluster.num_blocks();
-    if (ctas > 1) {  // each CTA adds up a part of the bins over all of them, into the first one's
-        cluster.sync();
-        const uint32_t each = 2 * kBinWords / ctas;  // (a whole number for 1, 2, 4, 8, 16)
-        for (uint32_t i = rank * each + threadIdx.x; i < (rank + 1) * each; i += kThreads) {
-            uint32_t sum = 0;
-#pragma unroll 4
-            for (uint32_t q = 0; q < ctas; ++q) sum += cluster.map_shared_rank(bin_n, q)[i];
-            cluster.map_shared_rank(bin_n, 0)[i] = sum;
-        }
-    }
+    merge_bins(bin_n, 2 * kBinWords);
     return s;
 }
 
@@ -572,9 +625,10 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
 template <typename T>
 __device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t op = sh.order[0], hi = sh.order[1], lo = sh.order[2], lane = threadIdx.x % 32;
-    uint64_t* first_list = cluster.map_shared_rank(reinterpret_cast<uint64_t*>(z.dynamic), 0);
-    uint32_t* first_count = cluster.map_shared_rank(&sh.count, 0);
+    const uint32_t op = sh.order[0], lane = threadIdx.x % 32;
+    const float from = value_of(sh.order[1]), least = value_of(sh.order[2]);
+    uint64_t* first_list = of_first(reinterpret_cast<uint64_t*>(z.dynamic));
+    uint32_t* first_count = of_first(&sh.count);
     const Weigh weigh{(double)max, z.c};
     Sum s{0, 0.0, 0.0};
     for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
@@ -588,11 +642,11 @@ __device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
             weigh.many(v + i, w);
 #pragma unroll
             for (int j = 0; j < kWeave; ++j) {
-                const uint32_t key = key_of(v[i + j]);
+                const float x = v[i + j];
                 all += w[j];
-                above += key >= hi ? w[j] : 0.0;
-                s.n += key >= hi;
-                mask |= (key >= lo) & (key < hi) ? 1u << (i + j) : 0u;
+                above += x >= from ? w[j] : 0.0;
+                s.n += x >= from;
+                mask |= (x >= least) & (x < from) ? 1u << (i + j) : 0u;
             }
         }
         s.lo += above, s.hi += all;
@@ -616,6 +670,8 @@ __device__ void perform(const Slice<T>& z, float max, Shared& sh) {
     Sum s{0, 0.0, 0.0};
     if (op == kCandidates)
         list_candidates(z, sh);
+    else if (op == kLevels)
+        count_levels(z, max, sh);
     else
         s = op == kHistogram ? histogram(z, max, sh) : gather(z, max, sh);
     s = block_scan(s, nullptr, sh);
@@ -788,8 +844,8 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     uint32_t* slots = again + kChunks;                                     // 4 kSlots words
     double* tile_sum = reinterpret_cast<double*>(slots + 4 * kSlots);      // a tile's
     float* chunk_max = reinterpret_cast<float*>(tile_sum + (tiles + 1) / 2 * 2);
-    double* first_sum = cluster.map_shared_rank(tile_sum, 0);
-    float* first_max = cluster.map_shared_rank(chunk_max, 0);
+    double* first_sum = of_first(tile_sum);
+    float* first_max = of_first(chunk_max);
 
     const uint32_t k = p.top_k == 0 || p.top_k > n ? n : p.top_k;
     const bool by_mass = p.top_p > 0.0f && p.top_p < 1.0f;
@@ -845,7 +901,6 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         if (threadIdx.x < ctas) {
             uint32_t* o = cluster.map_shared_rank(sh.order, threadIdx.x);
             o[0] = op, o[1] = hi, o[2] = lo, o[3] = shift;
-            if (op == kCandidates) *cluster.map_shared_rank(&sh.bound, threadIdx.x) = sh.bound;
         }
         all_sync();
     };
@@ -936,14 +991,14 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         low = block_min_float(low, sh);
         const uint32_t unit = min(mass_unit(chunks), 1u << 24);
         const uint64_t mass_goal = by_mass ? __double2ull_ru(fmin(reach_hi * unit, 0x1p40)) : ~0ull;
-        Bound bound{top, low < top ? fminf(255.9f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f, least, 0.0f, 1e30f, true};  // (halves: no overflow)
+        Bound bound{top, low < top ? fminf(255.9f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f, 0.0f, 1e30f};  // (halves: no overflow)
         // Where they do not fill either, a bound at 4.5 % of the maxima from below leaves about 3.1 elements a
         // chunk of 128 above it (3,700 at n = 151,936), whatever the values if they come in no order: a list that may
         // do, and shows it if it does.  It is tried where k is that small, or the mass above the bound seems to
         // be enough: if a share 1 - i / N of the chunks has nothing above x, -ln(1 - i / N) elements a chunk lie
         // there, so that the i-th largest maximum stands for N / (N - i) elements.
         const uint32_t most = (uint32_t)(n / kChunk * 0.955f);
-        bool guess = false;
+        bool guess = false, bounded = true;
         uint32_t reaching = 0;
         for (int round = 0; round < 2; ++round) {
             few_n[threadIdx.x] = 0, few_w[threadIdx.x] = 0;
@@ -979,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 if (guess) at = edge;
             }
             if (at == kAll) {  // not even all of them: every element from `least` up
-                bound.bounded = false;
+                bounded = false;
                 break;
             }
             if (bin == at) sh.count = upto;
@@ -992,24 +1047,32 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             if (reaching <= (guess ? most + 16 : k < chunks ? k + 32 : 64)) break;
             __syncthreads();
         }
-        guess &= !bound(least);  // (what passes `least` is all there is)
+        bounded = bounded && !bound(least);  // (or what passes `least` is all there is)
+        guess = guess && bounded;
+        float from = least;                                    // candidates: from here up
+        if (bounded) {
+            from = top;
+            for (uint32_t i = threadIdx.x; i < chunks; i += kThreads)
+                if (chunk_max[i] >= least && bound(chunk_max[i])) from = fminf(from, chunk_max[i]);
+            from = block_min_float(from, sh);
+        }
         __syncthreads();
-        if (threadIdx.x == 0) sh.count = 0, sh.chunks = 0, sh.bound = bound;
+        if (threadIdx.x == 0) sh.count = 0, sh.chunks = 0;
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < chunks; i += kThreads) {
-            if (!bound(chunk_max[i])) continue;
+            if (!(chunk_max[i] >= from)) continue;
             const uint32_t at = atomicAdd(&sh.chunks, 1u);
             if (at < kChunks) again[at] = i;
         }
         __syncthreads();
         // (without a bound the list would be the row)
-        reaching = bound.bounded || p.min_p > 0.0f || n <= kList ? sh.chunks : kAll;
+        reaching = bounded || p.min_p > 0.0f || n <= kList ? sh.chunks : kAll;
         if (reaching <= kChunks) {
-            if (ctas > 1 && reaching > kWarps * 4) {  // many chunks: all CTAs
-                command(kCandidates, reaching, 0, 0);
+            if (ctas > 1 && reaching > kWarps * 12) {  // many chunks: all CTAs
+                command(kCandidates, reaching, key_of(from), 0);
                 perform(slice, top, sh);
             } else {
-                if (threadIdx.x == 0) sh.order[1] = reaching;
+                if (threadIdx.x == 0) sh.order[1] = reaching, sh.order[2] = key_of(from);
                 __syncthreads();
                 list_candidates(slice, sh);  // (the first warps of all are this CTA's)
             }
@@ -1178,6 +1241,51 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         if (hi <= lo) lo = hi - 1;
         uint32_t inside = kAll;  // elements of [lo, hi)
         Sum base{0, 0.0, 0.0};   // count and mass from hi up
+        if (by_mass && hi - lo > 1) {
+            // levels of the weights' logarithm down to the lightest that may be kept
+            const float steps = fminf((float)(kBins - 8) / (top - value_of(lo)), 0x1p100f);
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < kBinWords; i += kThreads) bin_n[i] = 0;
+            command(kLevels, __float_as_uint(steps), 0, 0);
+            perform(slice, top, sh);
+            const float octaves = (float)c / steps;  // of a level
+            // (a level's weights lie within half of one of its middle, but for the roundings of 32 bits)
+            const double off = (double)exp2f(0.501f * octaves) - 1.0 + 0x1p-14;
+            Sum s{0, 0.0, 0.0}, before;
+            auto add_level = [&](uint32_t b, Sum* run) {
+                const uint32_t m = bin_n[bin_place(b)];
+                run->n += m, run->lo += (double)m * (double)exp2f(-(float)b * octaves);
+            };
+            for (uint32_t i = 0; i < kEachBin; ++i) add_level(threadIdx.x * kEachBin + i, &s);
+            block_scan(s, &before, sh);
+            uint32_t a = kBins - 1, z1 = kBins - 1;
+            for (uint32_t i = 0; i < kEachBin; ++i) {
+                const uint32_t b = threadIdx.x * kEachBin + i;
+                add_level(b, &before);
+                if ((before.n >= k || before.lo * (1.0 + off) >= reach_lo) && b < a) a = b;
+                if ((before.n >= k || before.lo * (1.0 - off) >= reach_hi) && b < z1) z1 = b;
+            }
+            const uint32_t last = min(level_of(value_of(lo), top, steps), kBins - 1);  // (nothing fills: the lightest)
+            a = min(block_min(a, sh), last), z1 = min(block_min(z1, sh), last);
+            s = Sum{0, 0.0, 0.0};
+            for (uint32_t b = a + threadIdx.x; b <= z1; b += kThreads) s.n += bin_n[bin_place(b)];
+            inside = block_scan(s, nullptr, sh).n;
+            // the levels' ends as keys: the lowest key of a level up to `level`
+            auto lowest = [&](uint32_t level) {
+                uint32_t under = kLowest - 1, from = hi - 1;  // (the maximum is of level 0)
+                while (from - under > 1) {
+                    const uint32_t mid = under + (from - under) / 2;
+                    if (level_of(value_of(mid), top, steps) <= level)
+                        from = mid;
+                    else
+                        under = mid;
+                }
+                return from;
+            };
+            lo = max(lo, lowest(z1));
+            if (a > 0) hi = lowest(a - 1);
+            if (hi <= lo) lo = hi - 1;
+        }
         for (int round = 0; round < 3 && inside > kList && (hi - lo > 1 || round == 0); ++round) {
             const uint32_t range = hi - lo;
             const uint32_t bits = 32 - __clz(range - 1 | 1);
@@ -1396,10 +1504,11 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
         if (e != cudaSuccess) return lrs_call_error(LRS_E_CUDA, "lrs_draw_device: %s", cudaGetErrorString(e));
         sms[dev] = count;
     }
-    // CTAs a row: as many as fill four an SM, no more than give each warp a tile
+    // CTAs a row: as many as give two an SM (three fit; with four the
+    // clusters' packing cost more than it gave: 64 x 151,936 in 41 us and not 25), no more than give each warp a tile
     const uint32_t tiles = (g.n + 15 + kTile - 1) / kTile;
     uint32_t ctas = 1;
-    while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 4 * (uint64_t)sms[dev] && ctas * kWarps < tiles) ctas *= 2;
+    while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 2 * (uint64_t)sms[dev] && ctas * kWarps < tiles) ctas *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(rows * ctas);
     cfg.blockDim = dim3(kThreads);
