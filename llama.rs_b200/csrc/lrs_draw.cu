@@ -21,6 +21,7 @@
 //      then inside one tile.  Without any filter step 1 sums in 64 bits and goes there directly.
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -93,6 +94,9 @@ __device__ __forceinline__ double power2(double y) {
     power2(in, out);
     return out[0];
 }
+
+// c as a float that 0 can be multiplied by (temperatures below 1e-38 make it larger than any).
+__device__ __forceinline__ float finite_float(double c) { return (float)fmin(c, 1e38); }
 
 struct Sum {
     uint32_t n;
@@ -478,7 +482,7 @@ __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
     uint32_t* first_count = of_first(&sh.count);
     const float least = value_of(sh.order[2]);
     const uint32_t reaching = sh.order[1], lane = threadIdx.x % 32;
-    const uint32_t step = cluster.num_blocks() * kWarps * kGroup;
+    const uint32_t step = sh.order[3] * kWarps * kGroup;  // (CTAs that share the chunks)
     uint32_t i = (cluster.block_rank() * kWarps + threadIdx.x / 32) * kGroup;
     auto load = [&](uint32_t first, uint32_t (&from)[kGroup], float (&v)[4 * kGroup]) {
         bool whole_chunks = true;
@@ -586,7 +590,7 @@ __device__ __noinline__ Sum histogram(const Slice<T>& z, float max, Shared& sh) 
         __syncthreads();
     }
     const Weigh weigh{(double)max, z.c};
-    const float cf = (float)z.c, scale = (float)min(mass_unit(z.n), 1u << 22);
+    const float cf = finite_float(z.c), scale = (float)min(mass_unit(z.n), 1u << 22);
     Sum s{0, 0.0, 0.0};
     for (uint32_t t = z.t0 + threadIdx.x / 32; t < z.t1; t += kWarps) {
         float v[32];
@@ -1069,12 +1073,12 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         reaching = bounded || p.min_p > 0.0f || n <= kList ? sh.chunks : kAll;
         if (reaching <= kChunks) {
             if (ctas > 1 && reaching > kWarps * 12) {  // many chunks: all CTAs
-                command(kCandidates, reaching, key_of(from), 0);
+                command(kCandidates, reaching, key_of(from), ctas);
                 perform(slice, top, sh);
             } else {
-                if (threadIdx.x == 0) sh.order[1] = reaching, sh.order[2] = key_of(from);
+                if (threadIdx.x == 0) sh.order[1] = reaching, sh.order[2] = key_of(from), sh.order[3] = 1;
                 __syncthreads();
-                list_candidates(slice, sh);  // (the first warps of all are this CTA's)
+                list_candidates(slice, sh);
             }
             __syncthreads();
             const uint32_t count = sh.count;
@@ -1241,14 +1245,14 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         if (hi <= lo) lo = hi - 1;
         uint32_t inside = kAll;  // elements of [lo, hi)
         Sum base{0, 0.0, 0.0};   // count and mass from hi up
-        if (by_mass && hi - lo > 1) {
-            // levels of the weights' logarithm down to the lightest that may be kept
-            const float steps = fminf((float)(kBins - 8) / (top - value_of(lo)), 0x1p100f);
+        // levels of the weights' logarithm down to the lightest that may be kept, where those are fine ones
+        const float steps = fminf((float)(kBins - 8) / (top - value_of(lo)), 0x1p100f);
+        const float octaves = finite_float(c) / steps;  // of a level
+        if (by_mass && hi - lo > 1 && octaves <= 1.0f) {
             __syncthreads();
             for (uint32_t i = threadIdx.x; i < kBinWords; i += kThreads) bin_n[i] = 0;
             command(kLevels, __float_as_uint(steps), 0, 0);
             perform(slice, top, sh);
-            const float octaves = (float)c / steps;  // of a level
             // (a level's weights lie within half of one of its middle, but for the roundings of 32 bits)
             const double off = (double)exp2f(0.501f * octaves) - 1.0 + 0x1p-14;
             Sum s{0, 0.0, 0.0}, before;
@@ -1297,7 +1301,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             base = total();
             // where the cut may lie: counts are exact, masses within their rounding (half a unit an
             // element, and the 32-bit power), Z within its own; masses here in 2^-40
-            const float cf = (float)c;
+            const float cf = finite_float(c);
             const int unit = 31 - __clz(min(mass_unit(n), 1u << 22));  // a bin's masses are in 2^(edge - unit)
             auto fixed = [](double mass) { return __double2ull_rd(fmin(fmax(mass, 0.0) * 0x1p40, 0x1p63)); };
             auto bin = [&](uint32_t b, uint64_t* lo_mass, uint64_t* hi_mass) {
@@ -1490,7 +1494,7 @@ size_t shared_bytes(uint32_t n) {
 template <typename T>
 int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     int dev = 0;
-    static int sms[kMaxDevices];  // (every thread that fills an entry writes the same value)
+    static std::atomic<int> sms[kMaxDevices];  // (every thread that fills an entry writes the same value)
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
         return lrs_call_error(LRS_E_CUDA, "lrs_draw_device: no current device");
     auto* kernel = draw_kernel<T>;
@@ -1508,7 +1512,7 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     // clusters' packing cost more than it gave: 64 x 151,936 in 41 us and not 25), no more than give each warp a tile
     const uint32_t tiles = (g.n + 15 + kTile - 1) / kTile;
     uint32_t ctas = 1;
-    while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 2 * (uint64_t)sms[dev] && ctas * kWarps < tiles) ctas *= 2;
+    while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 2 * (uint64_t)sms[dev].load() && ctas * kWarps < tiles) ctas *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(rows * ctas);
     cfg.blockDim = dim3(kThreads);

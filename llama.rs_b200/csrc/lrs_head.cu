@@ -17,6 +17,8 @@
 //           logits go out through shared memory, 64 bytes of a row at a time.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "lrs_ops.cuh"
 
 namespace {
@@ -516,7 +518,7 @@ bool code_map(CUtensorMap* m, const uint8_t* p, uint32_t rows, uint32_t k, uint6
 }
 
 struct DeviceInfo {
-    int sms = 0, smem = 0;
+    std::atomic<int> sms{0}, smem{0};  // (sms last: it says that both are there)
 };
 
 constexpr int kMaxDevices = 64;

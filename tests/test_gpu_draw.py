@@ -193,6 +193,41 @@ def test_uniforms_at_their_ends_and_tiny_filters():
     check(run(x, params, u), x.double().cpu().numpy(), params, u)
 
 
+@pytest.mark.parametrize("rows", [2, 40, 200])
+def test_long_rows_of_every_make(rows):
+    """Rows longer than a list, under every filter with many survivors: all alike (cut inside one run of
+    equal logits, at whole and half counts), two levels, sorted up and down, closed but for a few."""
+    import torch
+    rng = np.random.default_rng([14, rows])
+    n = 40960
+    kinds = [np.full(n, 2.5), np.where(np.arange(n) % 3 == 0, 1.0, -1.0), np.sort(rng.standard_normal(n) * 3),
+             np.sort(rng.standard_normal(n))[::-1], np.where(rng.random(n) < 0.999, -np.inf, rng.standard_normal(n)),
+             np.where(rng.random(n) < 0.5, -3e38, rng.standard_normal(n) * 0.1), rng.standard_normal(n) * 1e-20,
+             np.round(rng.standard_normal(n) * 4) / 4, rng.standard_cauchy(n)]
+    filters = [(1.0, 0, 0.5, 0.0), (1.0, 0, 0.25, 0.0), (1.0, 20480, 1.0, 0.0), (1.0, 5000, 0.9, 0.0), (1.0, 4097, 1.0, 0.0),
+               (1.0, 0, 1 - 2.0 ** -24, 0.0), (0.7, 0, 0.9999, 0.0), (2.0, 0, 1.0, 1e-30), (1.0, 0, 0.99, 1e-6),
+               (1.0, 3000, 0.999, 0.0), (1.0, 0, 1.0, 0.0), (1.0, 40959, 1.0, 0.0), (1.0, 0, 1e-30, 0.0)]
+    x = torch.from_numpy(np.stack([kinds[r % len(kinds)] for r in range(rows)])).float().cuda()
+    want = x.double().cpu().numpy()
+    for shift in range(0, len(filters), 1 if rows < 100 else 5):
+        params = records(rows, filters[shift:] + filters[:shift])
+        u = np.where(rng.random(rows) < 0.3, 0.5, rng.random(rows)).astype(np.float32)
+        check(run(x, params, u), want, params, u, shift)
+
+
+@pytest.mark.parametrize("t", [1e-45, 1e-39, 1e-20, 1e20, 3e38])
+def test_temperatures_of_long_rows(t):
+    import torch
+    rng = np.random.default_rng(15)
+    x = torch.from_numpy(matrix(rng, 10, 20000, "normal")).float().cuda()
+    x[3] *= 1e30
+    x[4] = 7.0
+    x[5, ::2] = -3e38
+    params = records(10, [(t, 0, 0.9, 0.0), (t, 5000, 1.0, 0.0), (t, 0, 0.5, 0.0), (t, 0, 1.0, 0.5), (t, 0, 1.0, 0.0), (t, 6000, 0.99, 0.0)])
+    u = rng.random(10, np.float32)
+    check(run(x, params, u), x.double().cpu().numpy(), params, u, t)
+
+
 def test_widest_row_and_offsets_past_32_bits():
     import torch
     rng = np.random.default_rng(10)
