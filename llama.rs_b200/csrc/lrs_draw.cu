@@ -271,6 +271,7 @@ struct Args {
     uint32_t* kept;
     int32_t* status;
     uint32_t n;
+    uint32_t twice;  // rows, where the grid goes over them twice (0: once)
 };
 
 // The row as this call sees it: element i at base[i + skew], base on a 16-byte boundary.
@@ -808,7 +809,10 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
-    const uint32_t r = blockIdx.x / ctas, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    uint32_t r = blockIdx.x / ctas;
+    const bool again_over = g.twice && r >= g.twice;
+    if (again_over) r -= g.twice;
     auto all_sync = [&] {
         if (ctas > 1)
             cluster.sync();
@@ -818,6 +822,9 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
 
     const lrs_draw_params p = g.params[r];
     const bool greedy = p.temperature <= 0.0f;
+    // (rows that may keep tens of thousands of tokens take several passes: they go first)
+    const bool deep = !greedy && (p.top_k == 0 || p.top_k > kList) && !(p.min_p > 0.0f);
+    if (g.twice && deep == again_over) return;
     const float u = greedy ? 0.0f : g.uniform[r];
     auto finish = [&](int32_t st, uint32_t token, double prob, uint32_t count) {
         g.tokens[r] = token;
@@ -1238,9 +1245,13 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             const double below = log2((double)p.min_p) / c;
             lo = max(lo, key_of(__double2float_rd((double)top + below - (fabs((double)top) - below) * 1e-12)));
         }
-        if (by_mass) {  // what is lighter than (1 - top_p) Z / n is left out even if every element is
-            const double below = log2((1.0 - top_p) * z * (1.0 - 2.0 * kApprox) / n) / c;
-            lo = max(lo, key_of(__double2float_rd((double)top + below - (fabs((double)top) + fabs(below)) * 1e-12)));
+        const double rest = (1.0 - top_p) * z;  // what may be left out
+        bool all_below = true;                  // min_p leaves out no more than that
+        if (by_mass) {  // what is lighter than rest / n is left out even if every element is; 2^-10 of that for the levels
+            const double below = log2(rest * (1.0 - 2.0 * kApprox) * 0x1p-10 / n) / c;
+            const uint32_t lightest = key_of(__double2float_rd((double)top + below - (fabs((double)top) + fabs(below)) * 1e-12));
+            all_below = lightest >= lo;
+            lo = max(lo, lightest);
         }
         if (hi <= lo) lo = hi - 1;
         uint32_t inside = kAll;  // elements of [lo, hi)
@@ -1261,13 +1272,20 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 run->n += m, run->lo += (double)m * (double)exp2f(-(float)b * octaves);
             };
             for (uint32_t i = 0; i < kEachBin; ++i) add_level(threadIdx.x * kEachBin + i, &s);
-            block_scan(s, &before, sh);
+            const double counted = block_scan(s, &before, sh).lo;
             uint32_t a = kBins - 1, z1 = kBins - 1;
             for (uint32_t i = 0; i < kEachBin; ++i) {
                 const uint32_t b = threadIdx.x * kEachBin + i;
                 add_level(b, &before);
-                if ((before.n >= k || before.lo * (1.0 + off) >= reach_lo) && b < a) a = b;
-                if ((before.n >= k || before.lo * (1.0 - off) >= reach_hi) && b < z1) z1 = b;
+                // (the mass above against top_p Z, and the mass below against the rest of Z: the one is good near
+                // the top, the other where top_p leaves little; what lies under the levels is 2^-10 of the rest, but
+                // for what min_p leaves out there: then only the first says that the cut is reached)
+                const double under = counted - before.lo;
+                const bool may = before.lo * (1.0 + off) >= reach_lo && under * (1.0 - off) <= rest * (1.0 + kApprox);
+                const bool does = before.lo * (1.0 - off) >= reach_hi ||
+                                  (all_below && under * (1.0 + off) + rest * 0x1p-9 <= rest * (1.0 - kApprox));
+                if ((before.n >= k || may) && b < a) a = b;
+                if ((before.n >= k || does) && b < z1) z1 = b;
             }
             const uint32_t last = min(level_of(value_of(lo), top, steps), kBins - 1);  // (nothing fills: the lightest)
             a = min(block_min(a, sh), last), z1 = min(block_min(z1, sh), last);
@@ -1513,8 +1531,14 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     const uint32_t tiles = (g.n + 15 + kTile - 1) / kTile;
     uint32_t ctas = 1;
     while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 2 * (uint64_t)sms[dev].load() && ctas * kWarps < tiles) ctas *= 2;
+    // Batches of several waves go over the rows twice, the heavy rows first, so that no such row is among the last
+    // to start: 1,024 x 151,936 with mixed filters in 162 us and not 193.  The CTAs that find their row in the other
+    // half leave at once.  (With one wave all start together: the second half would only cost.)
+    const bool waves = ctas == 1 && rows > 3 * (uint32_t)sms[dev].load();
+    Args args = g;
+    args.twice = waves ? rows : 0;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(rows * ctas);
+    cfg.gridDim = dim3(waves ? 2 * rows : rows * ctas);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = shared_bytes<T>(g.n);
     cfg.stream = s;
@@ -1525,7 +1549,7 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     at[1].val.clusterSchedulingPolicyPreference = cudaClusterSchedulingPolicySpread;
     cfg.attrs = at;
     cfg.numAttrs = ctas > 1 ? 2 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
     return e == cudaSuccess ? LRS_OK : lrs_call_error(LRS_E_CUDA, "lrs_draw_device: launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -1546,7 +1570,7 @@ extern "C" int lrs_draw_device(const void* d_logits, int dtype, uint32_t rows, u
     if ((uintptr_t)d_logits % size || (uintptr_t)d_params % 4 || (uintptr_t)d_uniform % 4 || (uintptr_t)d_tokens % 4 ||
         (uintptr_t)d_probs % 4 || (uintptr_t)d_kept % 4 || (uintptr_t)d_status % 4)
         return lrs_call_error(LRS_E_INVALID, "lrs_draw_device: a buffer is not aligned to its type");
-    const Args g{d_logits, ld, d_params, d_uniform, d_tokens, d_probs, d_kept, d_status, n};
+    const Args g{d_logits, ld, d_params, d_uniform, d_tokens, d_probs, d_kept, d_status, n, 0};
     const cudaStream_t s = (cudaStream_t)stream;
     return dtype == LRS_F32 ? launch<float>(g, rows, s) : dtype == LRS_BF16 ? launch<__nv_bfloat16>(g, rows, s) : launch<__half>(g, rows, s);
 }
