@@ -39,6 +39,7 @@ constexpr uint32_t kList = 4096;       // candidates that are listed
 constexpr uint32_t kChunk = 128;       // elements of a chunk
 constexpr uint32_t kPer = kTile / kChunk;
 constexpr uint32_t kChunks = 2048;     // chunks that are read again for them
+constexpr uint32_t kDirect = kWarps * 12;  // chunks whose candidates are listed with their keys at once
 constexpr uint32_t kFew = kThreads;    // candidates that are ranked without a sort
 constexpr uint32_t kBins = 4096;
 constexpr uint32_t kMaxCluster = 16;
@@ -429,10 +430,8 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-// Appends the elements of the lanes' bit masks to the first CTA's list: one addition to its count a warp.
-template <int N, typename At>
-__device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const float (&v)[N], uint32_t mask, At index) {
-    if (!__any_sync(kAll, mask != 0)) return;
+// Room on the first CTA's list for the elements of the lanes' bit masks: one addition to its count a warp.
+__device__ __forceinline__ uint32_t reserve(uint32_t* count, uint32_t mask) {
     const uint32_t lane = threadIdx.x % 32, mine = __popc(mask);
     uint32_t inc = mine;
 #pragma unroll
@@ -442,13 +441,28 @@ __device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const fl
     }
     uint32_t at = 0;
     if (lane == 31) at = atomicAdd(count, inc);
-    at = __shfl_sync(kAll, at, 31) + inc - mine;
+    return __shfl_sync(kAll, at, 31) + inc - mine;
+}
+// Appends them.
+template <int N, typename At>
+__device__ __forceinline__ void append(uint64_t* list, uint32_t* count, const float (&v)[N], uint32_t mask, At index) {
+    if (!__any_sync(kAll, mask != 0)) return;
+    uint32_t at = reserve(count, mask);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const bool hit = mask >> i & 1;
         if (hit & (at < kList)) list[at] = (uint64_t)key_of(v[i]) << 32 | ~index(i);
         at += hit;
     }
+}
+// Appends their indices alone, for fill_list(): a turn a hit, where append() has one an element (with that one
+// the gathering pass of a row of 151,936 took 106 us and not 86, the list of 3,700 candidates 62 and not 36).
+template <typename At>
+__device__ __forceinline__ void append_indices(uint64_t* list, uint32_t* count, uint32_t mask, At index) {
+    if (!__any_sync(kAll, mask != 0)) return;
+    uint32_t at = reserve(count, mask);
+    for (; mask; mask &= mask - 1, ++at)
+        if (at < kList) list[at] = ~index(__ffs(mask) - 1);
 }
 
 // The first CTA's copy of shared memory (its own for itself: the cluster's window is slower).
@@ -472,8 +486,27 @@ struct Slice {
     }
 };
 
+// The keys of a list of indices (the first CTA).
+template <typename T>
+__device__ __noinline__ void fill_list(const RowView<T>& row, uint64_t* list, uint32_t count) {
+    constexpr uint32_t kAhead = 8;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads * kAhead) {
+        uint32_t low[kAhead];
+        T x[kAhead];
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a) low[a] = (uint32_t)list[i + a * kThreads < count ? i + a * kThreads : i];
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a) x[a] = row.base[~low[a] + row.skew];
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a)
+            if (i + a * kThreads < count) list[i + a * kThreads] = (uint64_t)key_of(to_float<T>(x[a])) << 32 | low[a];
+    }
+    __syncthreads();
+}
+
 // Candidates: the elements from `least` up, to the first CTA's list, from the chunks that it has listed
-// (shared out over all warps).  Four chunks at a time, the next four on their way meanwhile.
+// (shared out over all warps).  Four chunks at a time, the next four on their way meanwhile.  Of more than
+// kDirect chunks the indices alone are listed.
 template <typename T>
 __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
     constexpr uint32_t kGroup = 4;
@@ -513,7 +546,10 @@ __device__ __noinline__ void list_candidates(const Slice<T>& z, Shared& sh) {
         uint32_t mask = 0;
 #pragma unroll
         for (uint32_t q = 0; q < 4 * kGroup; ++q) mask |= (v[q] >= least) & (i + q / 4 < reaching) ? 1u << q : 0u;
-        append(first_list, first_count, v, mask, [&](int q) { return from[q / 4] + q % 4 - z.row.skew; });
+        if (reaching > kDirect)
+            append_indices(first_list, first_count, mask, [&](int q) { return again[i + q / 4] * kChunk + lane * 4 + q % 4 - z.row.skew; });
+        else
+            append(first_list, first_count, v, mask, [&](int q) { return from[q / 4] + q % 4 - z.row.skew; });
         if (next >= reaching) return;
         i = next;
 #pragma unroll
@@ -662,7 +698,7 @@ __device__ __noinline__ Sum gather(const Slice<T>& z, float max, Shared& sh) {
             const uint32_t ties = __reduce_add_sync(kAll, __popc(mask));
             if (lane == 0) reinterpret_cast<uint32_t*>(z.first_max)[t] = ties;
         } else {
-            append(first_list, first_count, v, mask, [&](int i) { return z.index(t, i); });
+            append_indices(first_list, first_count, mask, [&](int i) { return z.index(t, i); });
         }
     }
     return s;
@@ -1007,7 +1043,9 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         // chunk of 128 above it (3,700 at n = 151,936), whatever the values if they come in no order: a list that may
         // do, and shows it if it does.  It is tried where k is that small, or the mass above the bound seems to
         // be enough: if a share 1 - i / N of the chunks has nothing above x, -ln(1 - i / N) elements a chunk lie
-        // there, so that the i-th largest maximum stands for N / (N - i) elements.
+        // there, so that the i-th largest maximum stands for N / (N - i) elements.  "Enough" begins at 0.96 of the
+        // goal: at 0.90 rows whose nucleus is a little too long listed in vain (1,024 x 151,936, sigma 3, top_p 0.9 in
+        // 842 us, 670 at 0.98), at 0.98 rows that would do went on (Zipf-like, top_p 0.85-0.95: 272 us, 199 at 0.94).
         const uint32_t most = (uint32_t)(n / kChunk * 0.955f);
         bool guess = false, bounded = true;
         uint32_t reaching = 0;
@@ -1041,7 +1079,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 const uint32_t edge = block_min(upto >= most ? bin : kAll, sh);
                 Sum held{0, 0.0, 0.0};
                 if (bin <= edge) held.lo = few_w[bin] * ((double)chunks / (chunks - min(before_n + few_n[bin] / 2, chunks - 1)));
-                guess = k <= kList * 7 / 8 || (by_mass && block_scan(held, nullptr, sh).lo >= 0.9 * (double)mass_goal);
+                guess = k <= kList * 7 / 8 || (by_mass && block_scan(held, nullptr, sh).lo >= 0.96 * (double)mass_goal);
                 if (guess) at = edge;
             }
             if (at == kAll) {  // not even all of them: every element from `least` up
@@ -1079,7 +1117,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         // (without a bound the list would be the row)
         reaching = bounded || p.min_p > 0.0f || n <= kList ? sh.chunks : kAll;
         if (reaching <= kChunks) {
-            if (ctas > 1 && reaching > kWarps * 12) {  // many chunks: all CTAs
+            if (ctas > 1 && reaching > kDirect) {  // many chunks: all CTAs
                 command(kCandidates, reaching, key_of(from), ctas);
                 perform(slice, top, sh);
             } else {
@@ -1089,6 +1127,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             }
             __syncthreads();
             const uint32_t count = sh.count;
+            if (reaching > kDirect && count <= kList) fill_list(row, list, count);
             auto row_mass = [&] {  // Z again, in 64 bits
                 Sum s{0, 0.0, 0.0};
                 for (uint32_t t = warp; t < tiles; t += kWarps) {
@@ -1418,6 +1457,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
             }
         } else {
             const uint32_t count = min(sh.count, kList);
+            fill_list(row, list, count);
             drop_light(count);
             const Cut end = find_cut(list, slots, again, count, above.n, above.lo, k, by_mass, reach, reach, weigh, sh);
             cut = end.keep ? end.entry : (uint64_t)hi << 32;
