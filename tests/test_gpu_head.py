@@ -155,6 +155,17 @@ def test_product_strides(dtype, rows, n, k, ldo, offset):
     within(product(a, sa, w, sw, dtype, ldo, offset), a, sa, w, sw, dtype, (rows, n, k, ldo))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,n,k,ldo,offset", [(65, 64, 100, 65, 0), (129, 256, 128, 259, 7), (130, 333, 200, 333, 1),
+                                                 (130, 333, 200, 338, 6), (131, 515, 140, 517, 5), (97, 640, 130, 644, 4), (200, 1281, 40, 1281, 3)])
+def test_product_rows_of_every_alignment(dtype, rows, n, k, ldo, offset):
+    """Row starts that walk through the 16-byte boundaries, whole and ragged runs of columns."""
+    rng = np.random.default_rng([rows, n, k, ldo, offset])
+    a, w = codes(rng, rows, k), codes(rng, n, k)
+    sa, sw = scales(rng, -(-k // 128), rows), scales(rng, -(-n // 128), -(-k // 128))
+    within(product(a, sa, w, sw, dtype, ldo, offset), a, sa, w, sw, dtype, (rows, n, k, ldo, offset))
+
+
 def test_product_of_exact_sums_is_exact():
     """Small whole numbers and scales of 1: every partial sum is exact in f32, so the product is too,
     whatever the order; each output then names its row, column and every block's part in it."""
