@@ -291,6 +291,7 @@ int  lrs_draw_device(const void* d_logits, int dtype, uint32_t rows, uint32_t n,
  *                      once to out_dtype.  d_out: row r at d_out + r * ld_out elements (ld_out >=
  *                      n, any alignment of the type).  Codes: d_a + r * ld_a and d_w + v * ld_w
  *                      bytes (>= k), bases and (of more than one row) ld_a, ld_w multiples of 16.
+ *                      A tile whose bounded waits ran out (about 2 s; none does in a sound launch) is NaN.
  * rows, n, k >= 1; rows, n <= 2^24, k <= 2^18 (LRS_E_INVALID otherwise; rows == 0 returns LRS_OK).
  * Enqueued on `stream` (cudaStream_t of the current device) without host synchronisation; no
  * state and no working memory is kept.  They return LRS_OK, LRS_E_INVALID or LRS_E_CUDA
