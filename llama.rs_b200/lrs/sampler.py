@@ -164,35 +164,43 @@ def dtype_code(t) -> int:
     return code
 
 
-_raw_stream = None
+_raw_stream = _raw_device = None
+
+
+def _raw_calls():
+    """torch's current stream and device by its own plain calls where it has them (a stream's handle in a tenth of
+    the time of building a Stream object)."""
+    global _raw_stream, _raw_device
+    import torch
+    _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
 def current_stream(device: int) -> int:
     """The handle of torch's current stream on a device."""
-    global _raw_stream
     if _raw_stream is None:
-        import torch
-        # (a tenth of the time of building a Stream object, where this torch has it)
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-            lambda d: torch.cuda.current_stream(d).cuda_stream)
+        _raw_calls()
     return _raw_stream(device)
 
 
 def launch(call, stream, args, *tensors) -> None:
     """Enqueues call(*args, stream handle) on the GPU of the tensors (None: absent), which have to lie on one: on
     torch's current stream there unless `stream` gives a handle.  Leaves the current device as it was."""
-    import torch
     device = tensors[0].get_device()
     if device < 0:
         raise SamplerError(LRS_E_INVALID, "CUDA tensors are needed")
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise SamplerError(LRS_E_INVALID, "the tensors lie on different devices")
+    if _raw_stream is None:
+        _raw_calls()
     if stream is None:
-        stream = current_stream(device)
-    if torch.cuda.current_device() == device:
+        stream = _raw_stream(device)
+    if _raw_device() == device:
         code = call(*args, stream)
     else:
+        import torch
         with torch.cuda.device(device):
             code = call(*args, stream)
     if code != LRS_OK:
