@@ -66,7 +66,7 @@ def fp8_logits(a, a_scales, w, w_scales, out, stream=None) -> None:
     """out (rows, n) = a (rows, k) times w (n, k) transposed, both e4m3 codes with the scales of
     quantize_rows and quantize_blocks; out is float32, bfloat16 or float16."""
     rows, k = _two(a, "a")
-    n, kb = w.shape[0], _blocks(k)
+    n, kb = _two(w, "w")[0], _blocks(k)
     launch(lib().lrs_fp8_logits, stream,
            (a.data_ptr(), _matrix(a, rows, k, 1, "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, 4, "a_scales"),
             w.data_ptr(), _matrix(w, n, k, 1, "w"), w_scales.data_ptr(),
@@ -86,7 +86,7 @@ class LmHead:
 
     def __init__(self, weight):
         import torch
-        n, k = weight.shape
+        n, k = _two(weight, "weight")
         self.vocab, self.k, self.device = n, k, weight.device
         self.codes = empty_codes(n, k, weight.device)
         self.scales = torch.empty(_blocks(n), _blocks(k), dtype=torch.float32, device=weight.device)
