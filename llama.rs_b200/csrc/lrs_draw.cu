@@ -1487,9 +1487,13 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     const double mass = block_scan(s, &before, sh).lo, target = (double)u * mass;
     uint32_t at = kAll, heavy = 0;
     double run = before.lo, base = 0.0;
+    // (a tile without weight holds nothing that is kept: a thread's `run` may exceed its neighbour's last one by a bit,
+    // since the sums before it are added in another order, and a target on that step would stop at such a tile)
     for (uint32_t t = i0; t < i1; ++t) {
-        if (tile_sum[t] > 0.0) heavy = t + 1;
-        if (at == kAll && run + tile_sum[t] > target) at = t, base = run;
+        if (tile_sum[t] > 0.0) {
+            heavy = t + 1;
+            if (at == kAll && run + tile_sum[t] > target) at = t, base = run;
+        }
         run += tile_sum[t];
     }
     uint32_t tile = block_min(at, sh);

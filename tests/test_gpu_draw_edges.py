@@ -1,0 +1,44 @@
+"""GPU tests of lrs_draw_device at the ends of its definition, against draw_ref.py: uniforms that fall on a
+step of the distribution function."""
+import numpy as np
+import pytest
+
+import lrs
+from test_gpu_draw import check, records, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("tiles,period,rows", [(128, 2, 64), (128, 2, 320), (149, 3, 64), (64, 2, 64), (40, 4, 16)])
+@pytest.mark.parametrize("filters", [(1.0, 0, 1.0, 0.0), (1.0, 30000, 1.0, 0.0), (1.0, 0, 0.96875, 0.0)])
+def test_uniforms_on_the_steps_between_closed_tiles(tiles, period, rows, filters):
+    """Tiles of 1024 elements with the same values in each open one and nothing in the others, and uniforms j /
+    64, which fall on the steps between tiles: there the sums of 64 bits decide by their last bit, so either
+    neighbour of the step (1e-13 of the mass around it) is right, but never a closed element or none."""
+    import torch
+    rng = np.random.default_rng([tiles, period, rows])
+    n = tiles * 1024
+    one = rng.standard_normal(1024)
+    x = np.where(np.arange(n) // 1024 % period == period - 1, np.tile(one, tiles), -np.inf).astype(np.float32)
+    params = records(rows, [filters])
+    u = (np.arange(rows) % 64 / 64).astype(np.float32)
+    tok, prob, kept, status = run(torch.from_numpy(x[None]).cuda(), params, u, ld=0)
+    assert (status == 0).all()
+    w = np.exp(x.astype(np.float64) - x.max())
+    order = np.argsort(-x, kind="stable")
+    keep = int(np.isfinite(x).sum()) if filters[1] == 0 else min(filters[1], int(np.isfinite(x).sum()))
+    if filters[2] < 1:
+        keep = int((np.cumsum(w[order]) < filters[2] * w.sum()).sum()) + 1
+        assert (np.abs(kept.astype(np.int64) - keep) <= 1).all()  # (top_p is on such a step as well)
+    else:
+        assert (kept == keep).all()
+    k = np.zeros(n)
+    k[order[:keep]] = w[order[:keep]]
+    c = np.cumsum(k)
+    # (the mass of one element is below 2^-14 of the whole; where the kept count is one off, so is the whole)
+    off = c[-1] * 1e-13 + (k[order[keep - 1]] * 2 if filters[2] < 1 else 0.0)
+    target = u.astype(np.float64) * c[-1]
+    assert (tok < n).all()
+    assert (k[tok] > 0).all()
+    assert (c[tok] >= target - off).all() and (c[tok] - k[tok] <= target + off).all()
+    assert (np.abs(prob - k[tok] / c[-1]) <= k[tok] / c[-1] * (2.0 ** -24 + 2.0 ** -38 + off / c[-1])).all()
