@@ -234,8 +234,13 @@ int  lrs_remap_tokens(const uint32_t* d_tokens, const int32_t* d_status, uint32_
  * No counterpart in the reference, whose sampler owns its generator and has no min-p: the
  * draw of a serving loop that brings its own random numbers (one uniform a row), on logits
  * of 32 or 16 bits.  Not bit-compatible with lrs_sample_device and not meant to be: here
- * the definition is over the real numbers, the kernels hold every weight and sum in 64 bits,
- * and the token is found in vocabulary order.  For row r, x = its logits, M = max x:
+ * the definition is over the real numbers, and the token is found in vocabulary order.  What
+ * decides is held in 64 bits: weights to 4e-14 of themselves (below 2^-1000 they are 0, and such
+ * an element is never drawn), sums as doubles or, of up to 4,096 listed elements, as whole numbers
+ * of 2^-51 of the largest weight, so that a result differs from the real-number one only where u
+ * or top_p falls within about 2e-12 of a step.  32-bit sums are used where both ends of their
+ * error (2^-20) give the same answer.  u = 0 draws the first kept element however light it is.
+ * For row r, x = its logits, M = max x:
  *   weights  w_i = exp((x_i - M) / temperature), Z = the sum of all w
  *   order    by x descending, equal x by ascending index
  *   kept     the shortest of these prefixes of the order: the first top_k elements (0, or

@@ -1,9 +1,9 @@
 // lrs_draw.cu — draws from given uniforms with temperature, top-k, top-p and min-p (sm_100a).
 //
 // The definition (include/llamars_sampler.h) is over the real numbers.  Every weight that decides
-// w = 2^((x - M) c), c = log2(e) / T, and every sum of them is held in 64 bits, so that a token
-// differs from the real-number one only where u falls within about 1e-13 of a step of the
-// distribution function.
+// w = 2^((x - M) c), c = log2(e) / T, and every sum of them is held in 64 bits (doubles, or whole
+// numbers of 2^-51 of the largest weight), so that a token differs from the real-number one only
+// where u falls within about 2e-12 of a step of the distribution function (1e-13 for doubles).
 //
 // A row is one cluster of CTAs (one CTA for batches, up to 16 for a few rows), each with a slice of
 // its tiles of 1024 elements; nothing is kept outside shared memory.
@@ -731,6 +731,12 @@ __device__ void perform(const Slice<T>& z, float max, Shared& sh) {
 __device__ __forceinline__ uint64_t units(const Weigh& weigh, uint64_t entry) {
     return __double2ull_rn(weigh(value_of((uint32_t)(entry >> 32))) * 0x1p51);
 }
+// The same where the token is found: one unit at least for every weight that is not 0, so that u = 0 draws the
+// first kept element however light it is (a list's 2^12 entries shift the steps by 2^-39 at most).
+__device__ __forceinline__ uint64_t drawn_units(double w) {
+    const uint64_t whole = __double2ull_rn(w * 0x1p51);
+    return whole == 0 && w > 0.0 ? 1 : whole;
+}
 // What of `reach` is left above `base`, in the same units.
 __device__ __forceinline__ uint64_t units_left(double reach, double base) {
     return __double2ull_ru(fmin(fmax(reach - base, 0.0) * 0x1p51, 0x1p63));
@@ -1015,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     const double top_p = (double)p.top_p;
     double reach_lo = by_mass ? top_p * z * (1.0 - kApprox) : INFINITY, reach_hi = by_mass ? top_p * z * (1.0 + kApprox) : INFINITY;
 
-    auto units_of = [&](uint64_t entry) { return units(weigh, entry); };
+    auto units_of = [&](uint64_t entry) { return drawn_units(weigh(value_of((uint32_t)(entry >> 32)))); };
     // Entries lighter than min_p leave the list.
     auto drop_light = [&](uint32_t count) {
         if (p.min_p > 0.0f) {
@@ -1175,7 +1181,8 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                     z = row_mass();
                     keep = kept_to(top_p * z);
                 }
-                if (real && part == 0) mass[me] = keep ? units : 0;
+                const uint64_t drawn = keep ? drawn_units(w) : 0;
+                if (real && part == 0) mass[me] = drawn;
                 const uint32_t kept = __syncthreads_count(keep && part == 0);
                 const uint32_t index = ~(uint32_t)entry;
                 uint64_t upto = 0, total = 0;
@@ -1189,9 +1196,9 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                     total += __shfl_xor_sync(kAll, total, o);
                     upto += __shfl_xor_sync(kAll, upto, o);
                 }
-                const bool passes = keep && units && (double)upto > (double)u * (double)total;
+                const bool passes = drawn && (double)upto > (double)u * (double)total;
                 uint32_t token = block_min(passes ? index : kAll, sh);
-                if (token == kAll) token = ~block_min(keep && units ? ~index : kAll, sh);  // (u's product rounded up: the last)
+                if (token == kAll) token = ~block_min(drawn ? ~index : kAll, sh);  // (u's product rounded up: the last)
                 if (real && part == 0 && index == token) finish(LRS_OK, token, w * 0x1p51 / (double)total, kept);
                 return leave();
             }
@@ -1231,7 +1238,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                             continue;
                         }
                         mine += round == 0;
-                        add_units(range + 3 * slot, __double2ull_rn(w * 0x1p51));
+                        add_units(range + 3 * slot, drawn_units(w));
                     }
                     __syncthreads();
                     const uint64_t a = read_units(range + 6 * threadIdx.x), b = read_units(range + 6 * threadIdx.x + 3);

@@ -42,3 +42,24 @@ def test_uniforms_on_the_steps_between_closed_tiles(tiles, period, rows, filters
     assert (k[tok] > 0).all()
     assert (c[tok] >= target - off).all() and (c[tok] - k[tok] <= target + off).all()
     assert (np.abs(prob - k[tok] / c[-1]) <= k[tok] / c[-1] * (2.0 ** -24 + 2.0 ** -38 + off / c[-1])).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 200])
+def test_the_lowest_uniform_takes_the_first_kept_element_however_light(rows):
+    """u = 0 draws the kept element of the lowest index, also where its weight is far below 2^-52 of the
+    row's: a few candidates, a list of them, a cut among many and no filter at all."""
+    import torch
+    few = np.full(3000, -50.0)
+    few[3], few[50] = -4.5, 0.0
+    listed = np.full(3000, -60.0)
+    listed[500:1499], listed[2500] = -40.0 - np.arange(999) % 7 * 0.125, 0.0
+    many = np.full(40960, -80.0)
+    many[7], many[2048:22047], many[30000] = -45.5, -44.0 - np.arange(19999) % 5 * 0.25, 0.0
+    plain = np.full(40960, -np.inf)
+    plain[9], plain[30000:] = -60.0, 0.0
+    for x, p, token in ((few, (0.1, 2, 1.0, 0.0), 3), (few, (0.1, 0, 1.0, 1e-20), 3), (listed, (1.0, 1000, 1.0, 0.0), 500),
+                        (listed, (1.0, 0, 1.0, 1e-20), 500), (many, (1.0, 20001, 1.0, 0.0), 7), (plain, (1.0, 0, 1.0, 0.0), 9)):
+        params, u = records(rows, [p]), np.zeros(rows, np.float32)
+        got = run(torch.from_numpy(x[None]).float().cuda(), params, u, ld=0)
+        check(got, [x] * rows, params, u, token)
+        assert (got[0] == token).all()
