@@ -63,3 +63,21 @@ def test_the_lowest_uniform_takes_the_first_kept_element_however_light(rows):
         got = run(torch.from_numpy(x[None]).float().cuda(), params, u, ld=0)
         check(got, [x] * rows, params, u, token)
         assert (got[0] == token).all()
+
+
+@pytest.mark.parametrize("rows", [2, 200])
+def test_a_cut_among_masses_below_the_histograms_unit(rows):
+    """One heavy element, and 40,959 of some 500 close values that weigh 2^-22 of it together, under the largest
+    top_p below 1: its cut lies among masses that no histogram resolves (Z is good to 2^-20 there), so that the
+    bracket is halved by exact sums until it fits the list."""
+    import torch
+    rng = np.random.default_rng([16, rows])
+    n = 40960
+    x = (-np.log(40959 * 2.0 ** 22) + rng.uniform(-5e-4, 5e-4, n)).astype(np.float32)
+    x[1234] = 0.0
+    assert 300 < len(np.unique(x)) < 1000
+    filters = [(1.0, 0, 1 - 2.0 ** -24, 0.0), (1.0, 30000, 1 - 2.0 ** -24, 0.0), (1.0, 0, 1 - 2.0 ** -23, 0.0)]
+    params, u = records(rows, filters), rng.random(rows, np.float32)
+    u[:2] = 0.0, 1 - 2.0 ** -24
+    got = run(torch.from_numpy(x[None]).cuda(), params, u, ld=0)
+    check(got, [x.astype(np.float64)] * rows, params, u)
