@@ -1605,8 +1605,7 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     at[1].val.clusterSchedulingPolicyPreference = cudaClusterSchedulingPolicySpread;
     cfg.attrs = at;
     cfg.numAttrs = ctas > 1 ? 2 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
-    return e == cudaSuccess ? LRS_OK : lrs_call_error(LRS_E_CUDA, "lrs_draw_device: launch failed: %s", cudaGetErrorString(e));
+    return launched("lrs_draw_device", cudaLaunchKernelEx(&cfg, kernel, args));
 }
 
 }  // namespace

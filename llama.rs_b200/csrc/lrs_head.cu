@@ -552,8 +552,7 @@ int launch(void (*kernel)(CUtensorMap, CUtensorMap, Args), DeviceInfo* info, con
     g.stages = ((uint32_t)info[dev].smem - 1024 - more) / g.stage_bytes;
     if (g.stages > kMaxStages) g.stages = kMaxStages;
     const uint32_t grid = g.tiles < (uint32_t)info[dev].sms ? g.tiles : (uint32_t)info[dev].sms;
-    kernel<<<grid, kThreads, g.stages * g.stage_bytes + 1024 + more, s>>>(first, second, g);
-    return launched("lrs_fp8_logits");
+    return launch_kernel("lrs_fp8_logits", kernel, grid, kThreads, g.stages * g.stage_bytes + 1024 + more, s, first, second, g);
 }
 
 template <typename T>

@@ -14,10 +14,21 @@ int lrs_call_error(int code, const char* fmt, ...);
 
 namespace lrs {
 
-// The call's launch result as a status.
-inline int launched(const char* what) {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? LRS_OK : lrs_call_error(LRS_E_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+// A launch's result as a status.  The runtime's last error is not asked: it may be that of an earlier call of this
+// thread; what a failed launch left there is taken away, since it is reported here.
+inline int launched(const char* what, cudaError_t e) {
+    if (e == cudaSuccess) return LRS_OK;
+    cudaGetLastError();
+    return lrs_call_error(LRS_E_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+}
+
+template <typename... P, typename... A>
+int launch_kernel(const char* what, void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
+                  const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    return launched(what, cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
 template <typename T>

@@ -223,29 +223,29 @@ int check(const char* what, const void* d_x, int dtype, uint32_t rows, uint32_t 
 }
 
 template <typename T, int VEC, bool ALIGNED>
-void launch_rows(const void* d_x, uint32_t rows, uint32_t k, uint64_t ld_x, uint8_t* d_q, uint64_t ld_q, float* d_scale,
+int launch_rows(const void* d_x, uint32_t rows, uint32_t k, uint64_t ld_x, uint8_t* d_q, uint64_t ld_q, float* d_scale,
                  uint64_t ld_scale, cudaStream_t s) {
     const uint32_t blocks = (k + kBlock - 1) / kBlock;
     const uint64_t units = (uint64_t)((rows + kRows - 1) / kRows) * blocks, per = kThreads / (kBlock / VEC);
-    quantize_rows_kernel<T, ALIGNED><<<(unsigned)((units + per - 1) / per), kThreads, 0, s>>>(
-        (const T*)d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, blocks, wide_codes<VEC>(d_q, ld_q));
+    return launch_kernel("lrs_quantize_rows", quantize_rows_kernel<T, ALIGNED>, (unsigned)((units + per - 1) / per), kThreads, 0, s,
+                         static_cast<const T*>(d_x), rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, blocks, wide_codes<VEC>(d_q, ld_q));
 }
 
 template <typename T, int VEC, bool ALIGNED>
-void launch_blocks(const void* d_x, uint32_t rows, uint32_t k, uint64_t ld_x, uint8_t* d_q, uint64_t ld_q,
-                   float* d_scale, uint64_t ld_scale, cudaStream_t s) {
+int launch_blocks(const void* d_x, uint32_t rows, uint32_t k, uint64_t ld_x, uint8_t* d_q, uint64_t ld_q,
+                  float* d_scale, uint64_t ld_scale, cudaStream_t s) {
     const uint32_t blocks = (k + kBlock - 1) / kBlock, tall = (rows + kBlock - 1) / kBlock;
-    quantize_blocks_kernel<T, ALIGNED><<<tall * blocks, 16 * sizeof(T) * 8, 0, s>>>(
-        (const T*)d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, blocks, wide_codes<VEC>(d_q, ld_q));
+    return launch_kernel("lrs_quantize_blocks", quantize_blocks_kernel<T, ALIGNED>, tall * blocks, 16 * sizeof(T) * 8, 0, s,
+                         static_cast<const T*>(d_x), rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, blocks, wide_codes<VEC>(d_q, ld_q));
 }
 
 template <typename T, int VEC>
-void launch_any(bool tall, const void* d_x, uint32_t rows, uint32_t k, uint64_t ld_x, uint8_t* d_q, uint64_t ld_q,
-                float* d_scale, uint64_t ld_scale, cudaStream_t s) {
+int launch_any(bool tall, const void* d_x, uint32_t rows, uint32_t k, uint64_t ld_x, uint8_t* d_q, uint64_t ld_q,
+               float* d_scale, uint64_t ld_scale, cudaStream_t s) {
     const bool aligned = (uintptr_t)d_x % 16 == 0 && (rows == 1 || ld_x * sizeof(T) % 16 == 0);
     auto run = tall ? aligned ? launch_blocks<T, VEC, true> : launch_blocks<T, VEC, false>
                     : aligned ? launch_rows<T, VEC, true> : launch_rows<T, VEC, false>;
-    run(d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, s);
+    return run(d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, s);
 }
 
 }  // namespace
@@ -256,8 +256,7 @@ extern "C" int lrs_quantize_rows(const void* d_x, int dtype, uint32_t rows, uint
     const int rc = check("lrs_quantize_rows", d_x, dtype, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, rows);
     if (rc != LRS_OK) return rc;
     auto run = dtype == LRS_F32 ? launch_any<float, 4> : dtype == LRS_BF16 ? launch_any<__nv_bfloat16, 8> : launch_any<__half, 8>;
-    run(false, d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, (cudaStream_t)stream);
-    return launched("lrs_quantize_rows");
+    return run(false, d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, (cudaStream_t)stream);
 }
 
 extern "C" int lrs_quantize_blocks(const void* d_x, int dtype, uint32_t rows, uint32_t k, uint64_t ld_x, uint8_t* d_q,
@@ -267,6 +266,5 @@ extern "C" int lrs_quantize_blocks(const void* d_x, int dtype, uint32_t rows, ui
                          ((uint64_t)k + kBlock - 1) / kBlock);
     if (rc != LRS_OK) return rc;
     auto run = dtype == LRS_F32 ? launch_any<float, 4> : dtype == LRS_BF16 ? launch_any<__nv_bfloat16, 8> : launch_any<__half, 8>;
-    run(true, d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, (cudaStream_t)stream);
-    return launched("lrs_quantize_blocks");
+    return run(true, d_x, rows, k, ld_x, d_q, ld_q, d_scale, ld_scale, (cudaStream_t)stream);
 }
