@@ -309,6 +309,15 @@ int  lrs_fp8_logits(const uint8_t* d_a, uint64_t ld_a, const float* d_a_scale, u
                     const uint8_t* d_w, uint64_t ld_w, const float* d_w_scale, uint64_t ld_ws,
                     uint32_t rows, uint32_t n, uint32_t k, void* d_out, int out_dtype, uint64_t ld_out,
                     void* stream);
+/* Test of the product's bounded waits (no counterpart in the reference): lrs_fp8_logits, but every
+ * CTA issues the copies of its first `steps` steps alone (a step: a tile's 128 columns; tile t is
+ * CTA t mod the CTAs'), and a wait takes `bound_cycles` SM cycles at most.  The waits for the next
+ * step run out, the tiles that it belongs to and all later ones of the CTA are NaN, and the launch
+ * ends; calls after it are not affected.                                              */
+int  lrs_test_fp8_logits_timeout(const uint8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint64_t ld_as,
+                                 const uint8_t* d_w, uint64_t ld_w, const float* d_w_scale, uint64_t ld_ws,
+                                 uint32_t rows, uint32_t n, uint32_t k, void* d_out, int out_dtype, uint64_t ld_out,
+                                 uint32_t steps, uint32_t bound_cycles, void* stream);
 
 /* ---- single-row drop-in (Sampler API) -------------------------------------------
  * lrs_sampler_new    replaces Sampler::new(seed)               (sampler.rs:33-37)

@@ -78,13 +78,13 @@ __device__ __forceinline__ bool elect() {
 }
 
 // Waits for a phase; false when the bound has passed or another warp has given up.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* lost) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long long bound, volatile uint32_t* lost) {
     if (bar_try(bar, parity)) return true;
     const long long t0 = clock64();
     do {
         if (bar_try(bar, parity)) return true;
         if (*lost) return false;
-    } while (clock64() - t0 < kWaitCycles);
+    } while (clock64() - t0 < bound);
     *lost = 1;
     return false;
 }
@@ -160,6 +160,8 @@ struct Args {
     uint32_t stages, buffers;          // of shared memory, of TMEM
     uint32_t columns, tmem_columns;    // of a buffer, allocated
     bool wide_out;                     // rows of d_out start on 16-byte boundaries
+    long long bound;                   // cycles that a wait takes at most
+    uint32_t copies;                   // steps that a CTA issues the copies of (all, but in the test of the waits)
 };
 
 struct Barriers {
@@ -226,10 +228,10 @@ __device__ __forceinline__ void copy_warp(const Args& g, Barriers& bars, uint32_
         const uint32_t r0 = t % g.row_tiles * g.tile_r, v0 = t / g.row_tiles * g.tile_v;
         const uint32_t y0 = weights_first ? v0 : r0, y1 = weights_first ? r0 : v0;
         for (uint32_t b = 0; b < g.blocks; ++b, ++issued) {
-            ok = bar_wait(empty + ring.at * 8, ring.turn ^ 1, lost);
+            ok = bar_wait(empty + ring.at * 8, ring.turn ^ 1, g.bound, lost);
             if (!ok) break;
             const uint32_t bar = full + ring.at * 8;
-            if (leader) {
+            if (leader && issued < g.copies) {
                 bar_expect(bar, g.stage_bytes);
                 tma_load(at, first, b * kBlock, y0, bar);
                 tma_load(at + g.first_bytes, second, b * kBlock, y1, bar);
@@ -238,7 +240,10 @@ __device__ __forceinline__ void copy_warp(const Args& g, Barriers& bars, uint32_
             at = ring.at == 0 ? base : at + g.stage_bytes;
         }
     }
-    if (!ok) {  // copies that a warp which gave up did not wait for land before the CTA ends
+    // every copy lands before the CTA ends, also where a warp that gave up did not wait for it (the lane that issued
+    // them counts them; before a stage's last copy came its `empty`, hence the ones before have landed)
+    if (leader) {
+        issued = min(issued, g.copies);
         for (uint32_t j = issued > g.stages ? issued - g.stages : 0; j < issued; ++j) {
             const long long t0 = clock64();
             while (!bar_try(full + j % g.stages * 8, j / g.stages & 1) && clock64() - t0 < kWaitCycles) {
@@ -260,7 +265,8 @@ __device__ __forceinline__ void mma_warp(const Args& g, Barriers& bars, uint32_t
     bool ok = true;
     for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
         for (uint32_t b = 0; b < g.blocks; ++b) {
-            ok = bar_wait(tempty + buffer.at * 8, buffer.turn ^ 1, lost) && bar_wait(full + ring.at * 8, ring.turn, lost);
+            ok = bar_wait(tempty + buffer.at * 8, buffer.turn ^ 1, g.bound, lost) &&
+                 bar_wait(full + ring.at * 8, ring.turn, g.bound, lost);
             if (!ok) break;
             tmem_fence_after();
             if (leader) {
@@ -305,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_consta
         for (uint32_t t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
             const uint32_t r0 = t % g.row_tiles * g.tile_r, v = t / g.row_tiles;
             for (uint32_t b = 0; b < g.blocks; ++b) {
-                ok = bar_wait(smem_of(&bars.sempty[ring.at]), ring.turn ^ 1, lost);
+                ok = bar_wait(smem_of(&bars.sempty[ring.at]), ring.turn ^ 1, g.bound, lost);
                 if (!ok) break;  // (a lane that gives up sends nothing more: the others run out as well)
                 const float* src = g.sa + b * g.ld_as + r0;
                 for (uint32_t c = lane; c < g.tile_r; c += 32) {
@@ -336,8 +342,8 @@ __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_consta
             for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
             // (after a wait that ran out the steps go on without waiting, and the tile is lost)
             for (uint32_t b = 0; b < g.blocks; ++b) {
-                ok &= bar_wait(smem_of(&bars.sfull[ring.at]), ring.turn, lost);
-                ok &= bar_wait(smem_of(&bars.tfull[buffer.at]), buffer.turn, lost);
+                ok &= bar_wait(smem_of(&bars.sfull[ring.at]), ring.turn, g.bound, lost);
+                ok &= bar_wait(smem_of(&bars.tfull[buffer.at]), buffer.turn, g.bound, lost);
                 __syncwarp();
                 tmem_fence_after();
                 float d[16];
@@ -361,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_consta
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[i] = fmaf(d[i], s[i], acc[i]);
             }
+            ok &= *lost == 0;  // (what ran on without waiting may have freed this warp's buffers early)
             T* out = reinterpret_cast<T*>(g.out) + (uint64_t)r0 * g.ld_out + v;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -423,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
                 const float s0 = a0 * w0;
                 a0 = a1, w0 = w1;
                 if (b + 2 < g.blocks) sa += g.ld_as, ++sw, a1 = __ldg(sa), w1 = __ldg(sw);
-                ok &= bar_wait(tfull + buffer * 8, turn, lost);
+                ok &= bar_wait(tfull + buffer * 8, turn, g.bound, lost);
                 __syncwarp();
                 tmem_fence_after();
                 const uint32_t from = lanes + buffer * kWideV;
@@ -442,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
                 buffer ^= 1;
                 turn ^= buffer == 0;
             }
+            ok &= *lost == 0;  // (what ran on without waiting may have freed this warp's buffers early)
             if (!ok) {
 #pragma unroll
                 for (int i = 0; i < (int)kWideCols; ++i) acc[i] = kLost;
@@ -579,11 +587,9 @@ int run(const uint8_t* d_a, uint64_t ld_a, const uint8_t* d_w, uint64_t ld_w, ui
                   : launch<T>(wide_kernel<T>, wide_info, ma, mw, g, kWideRegs, kWideWarps * 32 * kPiece, s);
 }
 
-}  // namespace
-
-extern "C" int lrs_fp8_logits(const uint8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint64_t ld_as,
-                              const uint8_t* d_w, uint64_t ld_w, const float* d_w_scale, uint64_t ld_ws, uint32_t rows,
-                              uint32_t n, uint32_t k, void* d_out, int out_dtype, uint64_t ld_out, void* stream) {
+int logits(const uint8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint64_t ld_as, const uint8_t* d_w, uint64_t ld_w,
+           const float* d_w_scale, uint64_t ld_ws, uint32_t rows, uint32_t n, uint32_t k, void* d_out, int out_dtype,
+           uint64_t ld_out, uint32_t copies, long long bound, void* stream) {
     if (rows == 0) return LRS_OK;
     if (out_dtype != LRS_F32 && out_dtype != LRS_BF16 && out_dtype != LRS_F16)
         return lrs_call_error(LRS_E_INVALID, "lrs_fp8_logits: out_dtype %d", out_dtype);
@@ -602,8 +608,27 @@ extern "C" int lrs_fp8_logits(const uint8_t* d_a, uint64_t ld_a, const float* d_
     g.sa = d_a_scale, g.sw = d_w_scale, g.out = d_out;
     g.ld_as = ld_as, g.ld_ws = ld_ws, g.ld_out = ld_out;
     g.rows = rows, g.n = n, g.blocks = (k + kBlock - 1) / kBlock;
+    g.copies = copies, g.bound = bound;
     const cudaStream_t s = (cudaStream_t)stream;
     return out_dtype == LRS_F32    ? run<float>(d_a, ld_a, d_w, ld_w, k, g, s)
            : out_dtype == LRS_BF16 ? run<__nv_bfloat16>(d_a, ld_a, d_w, ld_w, k, g, s)
                                    : run<__half>(d_a, ld_a, d_w, ld_w, k, g, s);
+}
+
+}  // namespace
+
+extern "C" int lrs_fp8_logits(const uint8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint64_t ld_as,
+                              const uint8_t* d_w, uint64_t ld_w, const float* d_w_scale, uint64_t ld_ws, uint32_t rows,
+                              uint32_t n, uint32_t k, void* d_out, int out_dtype, uint64_t ld_out, void* stream) {
+    return logits(d_a, ld_a, d_a_scale, ld_as, d_w, ld_w, d_w_scale, ld_ws, rows, n, k, d_out, out_dtype, ld_out, ~0u,
+                  kWaitCycles, stream);
+}
+
+extern "C" int lrs_test_fp8_logits_timeout(const uint8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint64_t ld_as,
+                                           const uint8_t* d_w, uint64_t ld_w, const float* d_w_scale, uint64_t ld_ws,
+                                           uint32_t rows, uint32_t n, uint32_t k, void* d_out, int out_dtype,
+                                           uint64_t ld_out, uint32_t steps, uint32_t bound_cycles, void* stream) {
+    if (bound_cycles == 0) return lrs_call_error(LRS_E_INVALID, "lrs_test_fp8_logits_timeout: bound is 0");
+    return logits(d_a, ld_a, d_a_scale, ld_as, d_w, ld_w, d_w_scale, ld_ws, rows, n, k, d_out, out_dtype, ld_out, steps,
+                  bound_cycles, stream);
 }

@@ -62,16 +62,23 @@ def quantize_blocks(x, codes, scales, stream=None) -> None:
     _quantize(lib().lrs_quantize_blocks, x, codes, scales, _blocks(rows), _blocks(k), stream)
 
 
+def _product(a, a_scales, w, w_scales, out) -> tuple:
+    rows, k = _two(a, "a")
+    n, kb = _two(w, "w")[0], _blocks(k)
+    return (a.data_ptr(), _matrix(a, rows, k, 1, "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, 4, "a_scales"),
+            w.data_ptr(), _matrix(w, n, k, 1, "w"), w_scales.data_ptr(), _matrix(w_scales, _blocks(n), kb, 4, "w_scales"),
+            rows, n, k, out.data_ptr(), dtype_code(out), _matrix(out, rows, n, 0, "out"))
+
+
 def fp8_logits(a, a_scales, w, w_scales, out, stream=None) -> None:
     """out (rows, n) = a (rows, k) times w (n, k) transposed, both e4m3 codes with the scales of
     quantize_rows and quantize_blocks; out is float32, bfloat16 or float16."""
-    rows, k = _two(a, "a")
-    n, kb = _two(w, "w")[0], _blocks(k)
-    launch(lib().lrs_fp8_logits, stream,
-           (a.data_ptr(), _matrix(a, rows, k, 1, "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, 4, "a_scales"),
-            w.data_ptr(), _matrix(w, n, k, 1, "w"), w_scales.data_ptr(),
-            _matrix(w_scales, _blocks(n), kb, 4, "w_scales"), rows, n, k, out.data_ptr(), dtype_code(out),
-            _matrix(out, rows, n, 0, "out")),
+    launch(lib().lrs_fp8_logits, stream, _product(a, a_scales, w, w_scales, out), a, a_scales, w, w_scales, out)
+
+
+def test_wait_timeout(a, a_scales, w, w_scales, out, steps: int, bound_cycles: int, stream=None) -> None:
+    """fp8_logits whose waits run out after every CTA's first `steps` steps (lrs_test_fp8_logits_timeout)."""
+    launch(lib().lrs_test_fp8_logits_timeout, stream, (*_product(a, a_scales, w, w_scales, out), steps, bound_cycles),
            a, a_scales, w, w_scales, out)
 
 

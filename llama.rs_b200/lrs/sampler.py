@@ -49,6 +49,7 @@ EXPORTS = [
     "lrs_sampler_state", "lrs_sampler_sample", "lrs_sample_device_noalloc", "lrs_assemble_shards",
     "lrs_poll_error", "lrs_noalloc_poll_error", "lrs_test_wait_timeout", "lrs_history_append",
     "lrs_remap_tokens", "lrs_draw_device", "lrs_quantize_rows", "lrs_quantize_blocks", "lrs_fp8_logits",
+    "lrs_test_fp8_logits_timeout",
 ]
 
 
@@ -109,6 +110,8 @@ def lib() -> ctypes.CDLL:
             f.restype = I
         L.lrs_fp8_logits.argtypes = [P, U64, P, U64, P, U64, P, U64, U32, U32, U32, P, I, U64, P]
         L.lrs_fp8_logits.restype = I
+        L.lrs_test_fp8_logits_timeout.argtypes = [*L.lrs_fp8_logits.argtypes[:-1], U32, U32, P]
+        L.lrs_test_fp8_logits_timeout.restype = I
         L.lrs_sampler_new.argtypes = [U64, I]
         L.lrs_sampler_new.restype = P
         L.lrs_sampler_free.argtypes = [P]
