@@ -13,16 +13,18 @@ cudaStream_t handle of that device) where one is given.
 """
 from __future__ import annotations
 
-from .sampler import LRS_E_INVALID, SamplerError, dtype_code, launch, lib
+from .sampler import LRS_E_INVALID, SamplerError, check_kind, dtype_code, launch, lib
 
 BLOCK = 128
 
 
-def _matrix(t, rows: int, cols: int, size: int, what: str) -> int:
-    """The leading dimension of a rows x cols tensor of contiguous rows and `size` bytes an element (0: any);
-    rows of one have none."""
-    if t.shape != (rows, cols) or (size and t.element_size() != size):
-        raise SamplerError(LRS_E_INVALID, f"{what}: a tensor of {rows} x {cols} is needed, of {size or 'any'} bytes an element")
+def _matrix(t, rows: int, cols: int, kind, what: str) -> int:
+    """The leading dimension of a rows x cols tensor of contiguous rows and a kind of type (check_kind; None: the
+    caller has looked); rows of one have none."""
+    if t.shape != (rows, cols):
+        raise SamplerError(LRS_E_INVALID, f"{what}: a tensor of {rows} x {cols} is needed")
+    if kind is not None:
+        check_kind(t, kind, what)
     step, inner = t.stride()
     if inner != 1 and cols > 1:
         raise SamplerError(LRS_E_INVALID, f"{what}: contiguous rows are needed")
@@ -42,8 +44,8 @@ def _two(t, what: str):
 def _quantize(call, x, codes, scales, a: int, b: int, stream) -> None:
     rows, k = x.shape
     launch(call, stream,
-           (x.data_ptr(), dtype_code(x), rows, k, _matrix(x, rows, k, 0, "x"), codes.data_ptr(),
-            _matrix(codes, rows, k, 1, "codes"), scales.data_ptr(), _matrix(scales, a, b, 4, "scales")),
+           (x.data_ptr(), dtype_code(x), rows, k, _matrix(x, rows, k, None, "x"), codes.data_ptr(),
+            _matrix(codes, rows, k, "codes", "codes"), scales.data_ptr(), _matrix(scales, a, b, "f32", "scales")),
            x, codes, scales)
 
 
@@ -65,9 +67,9 @@ def quantize_blocks(x, codes, scales, stream=None) -> None:
 def _product(a, a_scales, w, w_scales, out) -> tuple:
     rows, k = _two(a, "a")
     n, kb = _two(w, "w")[0], _blocks(k)
-    return (a.data_ptr(), _matrix(a, rows, k, 1, "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, 4, "a_scales"),
-            w.data_ptr(), _matrix(w, n, k, 1, "w"), w_scales.data_ptr(), _matrix(w_scales, _blocks(n), kb, 4, "w_scales"),
-            rows, n, k, out.data_ptr(), dtype_code(out), _matrix(out, rows, n, 0, "out"))
+    return (a.data_ptr(), _matrix(a, rows, k, "codes", "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, "f32", "a_scales"),
+            w.data_ptr(), _matrix(w, n, k, "codes", "w"), w_scales.data_ptr(), _matrix(w_scales, _blocks(n), kb, "f32", "w_scales"),
+            rows, n, k, out.data_ptr(), dtype_code(out), _matrix(out, rows, n, None, "out"))
 
 
 def fp8_logits(a, a_scales, w, w_scales, out, stream=None) -> None:

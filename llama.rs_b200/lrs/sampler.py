@@ -153,6 +153,7 @@ def _check(code: int, ctx=None):
 
 
 _dtype_codes = None
+_kinds: dict = {}
 
 
 def dtype_code(t) -> int:
@@ -165,6 +166,16 @@ def dtype_code(t) -> int:
     if code is None:
         raise SamplerError(LRS_E_INVALID, f"{t.dtype}: float32, bfloat16 or float16 is needed")
     return code
+
+
+def check_kind(t, kind: str, what: str) -> None:
+    """Refuses a tensor whose type is not of a kind: "codes" (e4m3 values or their bytes), "f32" or "i32"."""
+    if not _kinds:
+        import torch
+        _kinds.update(codes={torch.float8_e4m3fn, torch.uint8}, f32={torch.float32}, i32={torch.int32, torch.uint32})
+    if t.dtype not in _kinds[kind]:
+        names = {"codes": "float8_e4m3fn or uint8", "f32": "float32", "i32": "int32"}
+        raise SamplerError(LRS_E_INVALID, f"{what}: {t.dtype}, {names[kind]} is needed")
 
 
 _raw_stream = _raw_device = None
@@ -328,9 +339,12 @@ class BatchSampler:
             ld = step if have > 1 else n if rows <= 1 else 0
         if (rows > have and ld) or n > width or params.numel() * params.element_size() < 16 * rows:
             raise SamplerError(LRS_E_INVALID, f"draw_device: the logits or the parameters hold fewer than {rows} rows of {n}")
-        for t in (uniform, tokens, probs, kept, status):
-            if t is not None and (t.numel() < rows or t.element_size() != 4 or not t.is_contiguous()):
-                raise SamplerError(LRS_E_INVALID, f"draw_device: a buffer is not {rows} 32-bit values in a row")
+        for t, kind, what in ((uniform, "f32", "uniform"), (tokens, "i32", "tokens"), (probs, "f32", "probs"),
+                              (kept, "i32", "kept"), (status, "i32", "status")):
+            if t is not None:
+                check_kind(t, kind, what)
+                if t.numel() < rows or not t.is_contiguous():
+                    raise SamplerError(LRS_E_INVALID, f"{what}: not {rows} values in a row")
         if not params.is_contiguous():
             raise SamplerError(LRS_E_INVALID, "draw_device: the parameters are not contiguous")
         launch(lib().lrs_draw_device, stream,

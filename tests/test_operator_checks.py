@@ -15,3 +15,90 @@ def test_the_test_of_the_products_waits_checks_its_arguments(built_lib):
     assert lrs.lib().lrs_last_error(None) == b"lrs_test_fp8_logits_timeout: bound is 0"
     assert call(*args[:-1], 299, 1, 1000, None) == lrs.LRS_E_INVALID
     assert b"leading dimension" in lrs.lib().lrs_last_error(None)
+
+
+def refused(message, call, *args, **kw):
+    with pytest.raises(lrs.SamplerError, match=message) as e:
+        call(*args, **kw)
+    assert e.value.code == lrs.LRS_E_INVALID
+
+
+def draw_args(rows=2, n=100, **kw):
+    """draw_device's arguments, right but for lying on the CPU."""
+    import torch
+    a = dict(logits=torch.zeros(rows, n), params=torch.zeros(16 * rows, dtype=torch.uint8), uniform=torch.zeros(rows),
+             tokens=torch.zeros(rows, dtype=torch.int32), probs=torch.zeros(rows), kept=torch.zeros(rows, dtype=torch.int32),
+             status=torch.zeros(rows, dtype=torch.int32))
+    a.update(kw)
+    return a
+
+
+def product_args(rows=3, n=300, k=200):
+    import torch
+    return dict(a=lrs.empty_codes(rows, k, "cpu"), a_scales=torch.zeros(2, rows), w=lrs.empty_codes(n, k, "cpu"),
+                w_scales=torch.zeros(3, 2), out=torch.zeros(rows, n))
+
+
+def test_calls_on_the_cpu_get_as_far_as_the_device(built_lib):
+    """What the refusals below differ from."""
+    import torch
+    refused("CUDA tensors are needed", lrs.BatchSampler.draw_device, **draw_args())
+    refused("CUDA tensors are needed", lrs.BatchSampler.draw_device, **draw_args(tokens=torch.zeros(2, dtype=torch.uint32)))
+    refused("CUDA tensors are needed", lrs.fp8_logits, **product_args())
+    for call, scales in ((lrs.quantize_rows, (2, 3)), (lrs.quantize_blocks, (1, 2))):
+        for codes in (torch.zeros(3, 200, dtype=torch.uint8), lrs.empty_codes(3, 200, "cpu")):
+            refused("CUDA tensors are needed", call, torch.zeros(3, 200), codes, torch.zeros(scales))
+
+
+@pytest.mark.parametrize("name,dtype", [("uniform", "int32"), ("uniform", "float64"), ("tokens", "float32"), ("tokens", "int64"),
+                                        ("probs", "int32"), ("probs", "bfloat16"), ("kept", "float32"), ("status", "int16")])
+def test_a_draws_buffers_have_the_types_that_they_are_read_as(built_lib, name, dtype):
+    import torch
+    bad = torch.zeros(4, dtype=getattr(torch, dtype))
+    refused(f"{name}: torch.{dtype}, ", lrs.BatchSampler.draw_device, rows=2, **draw_args(**{name: bad}))
+
+
+@pytest.mark.parametrize("dtype", ["float8_e5m2", "int8", "bool", "float32"])
+def test_codes_are_e4m3(built_lib, dtype):
+    import torch
+    bad = lambda *shape: torch.zeros(shape, dtype=getattr(torch, dtype))
+    message = f"torch.{dtype}, float8_e4m3fn or uint8 is needed"
+    refused("codes: " + message, lrs.quantize_rows, torch.zeros(3, 200), bad(3, 200), torch.zeros(2, 3))
+    refused("codes: " + message, lrs.quantize_blocks, torch.zeros(3, 200), bad(3, 200), torch.zeros(1, 2))
+    refused("a: " + message, lrs.fp8_logits, **{**product_args(), "a": bad(3, 208)[:, :200]})
+    refused("w: " + message, lrs.fp8_logits, **{**product_args(), "w": bad(300, 208)[:, :200]})
+
+
+@pytest.mark.parametrize("dtype", ["int32", "float64", "bfloat16"])
+def test_scales_are_f32(built_lib, dtype):
+    import torch
+    bad = lambda *shape: torch.zeros(shape, dtype=getattr(torch, dtype))
+    message = f"scales: torch.{dtype}, float32 is needed"
+    refused(message, lrs.quantize_rows, torch.zeros(3, 200), lrs.empty_codes(3, 200, "cpu"), bad(2, 3))
+    refused(message, lrs.quantize_blocks, torch.zeros(3, 200), lrs.empty_codes(3, 200, "cpu"), bad(1, 2))
+    refused("a_" + message, lrs.fp8_logits, **{**product_args(), "a_scales": bad(2, 3)})
+    refused("w_" + message, lrs.fp8_logits, **{**product_args(), "w_scales": bad(3, 2)})
+
+
+def test_shapes_and_strides_are_named_where_they_are_wrong(built_lib):
+    import torch
+    f, z = torch.zeros, lambda *s: torch.zeros(s, dtype=torch.uint8)
+    draw = lrs.BatchSampler.draw_device
+    refused("logits: a 2-d tensor", draw, **draw_args(logits=f(200)))
+    refused("contiguous rows", draw, **draw_args(logits=f(100, 2).t()))
+    refused("contiguous rows", draw, **draw_args(logits=f(2, 200)[:, ::2]))
+    refused("fewer than 2 rows", draw, **draw_args(params=z(31)))
+    refused("parameters are not contiguous", draw, **draw_args(params=f(2, 8)[:, ::2]))
+    refused("uniform: not 2 values", draw, **draw_args(uniform=f(1)))
+    refused("kept: not 2 values", draw, **draw_args(kept=torch.zeros(4, dtype=torch.int32)[::2]))
+    refused("float64: float32, bfloat16 or float16", draw, **draw_args(logits=f(2, 100).double()))
+    refused("x: a 2-d tensor", lrs.quantize_rows, f(200), z(1, 200), f(2, 1))
+    refused("codes: a tensor of 3 x 200", lrs.quantize_rows, f(3, 200), z(3, 199), f(2, 3))
+    refused("scales: a tensor of 2 x 3", lrs.quantize_rows, f(3, 200), z(3, 200), f(3, 2))
+    refused("scales: a tensor of 1 x 2", lrs.quantize_blocks, f(3, 200), z(3, 200), f(2, 3))
+    refused("x: contiguous rows", lrs.quantize_blocks, f(200, 3).t(), z(3, 200), f(1, 2))
+    refused("float64: float32, bfloat16 or float16", lrs.quantize_rows, f(3, 200).double(), z(3, 200), f(2, 3))
+    refused("w: a tensor of 300 x 200", lrs.fp8_logits, **{**product_args(), "w": z(300, 199)})
+    refused("w_scales: a tensor of 3 x 2", lrs.fp8_logits, **{**product_args(), "w_scales": f(2, 3)})
+    refused("out: a tensor of 3 x 300", lrs.fp8_logits, **{**product_args(), "out": f(3, 301)})
+    refused("out: contiguous rows", lrs.fp8_logits, **{**product_args(), "out": f(300, 3).t()})
