@@ -38,7 +38,10 @@ def _blocks(k: int) -> int:
 def _two(t, what: str):
     if t.dim() != 2:
         raise SamplerError(LRS_E_INVALID, f"{what}: a 2-d tensor is needed")
-    return t.shape
+    rows, cols = t.shape
+    if rows >> 32 or cols >> 32:  # (ctypes would cut them)
+        raise SamplerError(LRS_E_INVALID, f"{what}: {rows} x {cols} is larger than 2^32 a side")
+    return rows, cols
 
 
 def _quantize(call, x, codes, scales, a: int, b: int, stream) -> None:

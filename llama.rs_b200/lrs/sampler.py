@@ -337,6 +337,9 @@ class BatchSampler:
         n = width if n is None else n
         if ld is None:
             ld = step if have > 1 else n if rows <= 1 else 0
+        # (sizes that ctypes would cut to 32 bits, and a given ld that leads past the tensor's last element)
+        if rows >> 32 or n >> 32 or ld < 0 or (rows > 1 and (rows - 1) * ld + n > (have - 1) * step + width):
+            raise SamplerError(LRS_E_INVALID, f"draw_device: {rows} rows of {n}, {ld} apart, do not lie within the logits")
         if (rows > have and ld) or n > width or params.numel() * params.element_size() < 16 * rows:
             raise SamplerError(LRS_E_INVALID, f"draw_device: the logits or the parameters hold fewer than {rows} rows of {n}")
         for t, kind, what in ((uniform, "f32", "uniform"), (tokens, "i32", "tokens"), (probs, "f32", "probs"),

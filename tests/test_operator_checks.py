@@ -102,3 +102,33 @@ def test_shapes_and_strides_are_named_where_they_are_wrong(built_lib):
     refused("w_scales: a tensor of 3 x 2", lrs.fp8_logits, **{**product_args(), "w_scales": f(2, 3)})
     refused("out: a tensor of 3 x 300", lrs.fp8_logits, **{**product_args(), "out": f(3, 301)})
     refused("out: contiguous rows", lrs.fp8_logits, **{**product_args(), "out": f(300, 3).t()})
+
+
+def test_a_leading_dimension_stays_within_the_tensor(built_lib):
+    import torch
+    draw, padded = lrs.BatchSampler.draw_device, torch.zeros(4, 128)[:, :100]
+    for rows, kw in ((4, dict(ld=129)), (4, dict(ld=1 << 40)), (4, dict(ld=-128)), (1, dict(ld=-1)), (2, dict(ld=385, n=100)),
+                     (5, dict()), (5, dict(ld=128)), (4, dict(ld=100)), (4, dict(n=101)), (4, dict(n=-1)),
+                     (4, dict(n=(1 << 32) + 5)), (-1, dict()), (-(1 << 32) + 4, dict())):
+        if (rows, kw) == (4, dict(ld=100)):  # (rows closer together than the tensor's are within it)
+            refused("CUDA tensors are needed", draw, **draw_args(4, logits=padded), rows=rows, **kw)
+            continue
+        refused("draw_device: ", draw, **draw_args(8, logits=padded), rows=rows, **kw)
+    # what the last row reaches, and row 0 for every row
+    for rows, kw in ((4, dict(ld=128)), (2, dict(ld=384)), (2, dict(ld=384, n=7)), (2, dict(ld=477, n=7)), (9, dict(ld=0)),
+                     (1, dict(ld=1 << 40)), (0, dict()), (0, dict(ld=1 << 40))):
+        refused("CUDA tensors are needed", draw, **draw_args(9, logits=padded), rows=rows, **kw)
+    refused("draw_device: ", draw, **draw_args(9, logits=padded), rows=2, ld=478, n=7)
+
+
+def test_sizes_past_32_bits_are_refused(built_lib):
+    """They would reach the library cut to 32 bits."""
+    import torch
+    tall, long, u8 = (1 << 32) + 3, (1 << 32) + 200, torch.uint8
+    for call in (lrs.quantize_rows, lrs.quantize_blocks):
+        for shape in ((tall, 1), (3, long)):
+            refused("larger than 2\\^32", call, torch.zeros(1, 1).expand(shape), torch.zeros(1, 1, dtype=u8).expand(shape), torch.zeros(1, 1))
+    a = product_args()
+    refused("larger than 2\\^32", lrs.fp8_logits, **{**a, "w": torch.zeros(1, 1, dtype=u8).expand(tall, 200)})
+    refused("larger than 2\\^32", lrs.fp8_logits, **{**a, "a": torch.zeros(1, 1, dtype=u8).expand(tall, 200)})
+    refused("draw_device: ", lrs.BatchSampler.draw_device, **draw_args(logits=torch.empty(2, long, device="meta")))
