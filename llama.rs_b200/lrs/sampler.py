@@ -365,11 +365,24 @@ class BatchSampler:
                                  rows=hidden.shape[0])
         return logits
 
+    def check_head(self, head) -> None:
+        """Refuses a head on another device than the sampler's (its stream would meet this context there)."""
+        if head.device.type != "cuda" or head.device.index != self.device:
+            raise SamplerError(LRS_E_INVALID, f"the head lies on {head.device}, the sampler on cuda:{self.device}")
+
     def sample_hidden(self, head, hidden, params, state, tokens, hist=None, hist_len=None, probs=None, status=None):
-        """The same with the exact sampler: the head's logits of the hidden states, then sample_device."""
+        """The same with the exact sampler: the head's logits of the hidden states, then sample_device.  The head lies
+        on the sampler's device, and every buffer holds a row for each hidden state."""
+        self.check_head(head)
+        rows = hidden.shape[0]
+        for t, size, what in ((params, PARAMS_DTYPE.itemsize, "params"), (state, 8, "state"), (tokens, 4, "tokens"),
+                              (hist_len, 4, "hist_len"), (probs, 4, "probs"), (status, 4, "status")):
+            if t is not None and t.numel() * t.element_size() < size * rows:
+                raise SamplerError(LRS_E_INVALID, f"{what}: fewer than {rows} rows")
+        if hist is not None and hist.shape[0] < rows:
+            raise SamplerError(LRS_E_INVALID, f"hist: fewer than {rows} rows")
         logits = head.logits(hidden)
-        self.sample_device(logits, params, state, tokens, hist=hist, hist_len=hist_len, probs=probs, status=status,
-                           rows=hidden.shape[0])
+        self.sample_device(logits, params, state, tokens, hist=hist, hist_len=hist_len, probs=probs, status=status, rows=rows)
         return logits
 
     @staticmethod

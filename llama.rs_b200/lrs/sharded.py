@@ -214,6 +214,7 @@ class VocabShardedSampler:
         rows of the weights, `hidden` (rows, k) every row's hidden states.  On torch's current stream."""
         if head.vocab != self.shard_n or hidden.shape[0] != self.rows:
             raise ValueError(f"a head of {self.shard_n} tokens and {self.rows} hidden states are needed")
+        self.bs.check_head(head)
         self.sample(head.logits(hidden), params, state, tokens, hist=hist, hist_len=hist_len, probs=probs,
                     status=status)
 

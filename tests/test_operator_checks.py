@@ -132,3 +132,65 @@ def test_sizes_past_32_bits_are_refused(built_lib):
     refused("larger than 2\\^32", lrs.fp8_logits, **{**a, "w": torch.zeros(1, 1, dtype=u8).expand(tall, 200)})
     refused("larger than 2\\^32", lrs.fp8_logits, **{**a, "a": torch.zeros(1, 1, dtype=u8).expand(tall, 200)})
     refused("draw_device: ", lrs.BatchSampler.draw_device, **draw_args(logits=torch.empty(2, long, device="meta")))
+
+
+class StandInHead:
+    """A head of 5 tokens on a device of one's choice."""
+    vocab = 5
+
+    def __init__(self, device):
+        import torch
+        self.device = torch.device(device)
+
+    def logits(self, hidden, out=None, dtype=None):
+        import torch
+        return torch.zeros(hidden.shape[0], self.vocab, device="meta")
+
+
+def sampler_without_a_gpu(device=0):
+    bs = lrs.BatchSampler.__new__(lrs.BatchSampler)
+    bs._h, bs.device, bs.calls = None, device, []
+    bs.sample_device = lambda *args, **kw: bs.calls.append((args, kw))
+    return bs
+
+
+def hidden_args(rows=3, **kw):
+    """sample_hidden's arguments (meta tensors: only shapes and devices count)."""
+    import torch
+    t = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device="meta")
+    a = dict(hidden=t(rows, 8, dtype=torch.float32), params=t(rows * 24, dtype=torch.uint8), state=t(rows, dtype=torch.int64),
+             tokens=t(rows), hist=t(rows, 16), hist_len=t(rows), probs=t(rows, dtype=torch.float32), status=t(rows))
+    a.update(kw)
+    return a
+
+
+def test_the_head_and_the_sampler_lie_on_one_device(built_lib):
+    import torch
+    from lrs.sharded import VocabShardedSampler
+    bs = sampler_without_a_gpu(0)
+    refused("the head lies on cuda:1, the sampler on cuda:0", bs.sample_hidden, StandInHead("cuda:1"), **hidden_args())
+    refused("the head lies on cpu, the sampler on cuda:0", bs.sample_hidden, StandInHead("cpu"), **hidden_args())
+    vs = VocabShardedSampler.__new__(VocabShardedSampler)
+    vs.shard_n, vs.rows, vs.bs, vs.calls = 5, 3, bs, []
+    vs.sample = lambda *args, **kw: vs.calls.append(args)
+    a = hidden_args()
+    refused("the head lies on cuda:1, the sampler on cuda:0", vs.sample_hidden, StandInHead("cuda:1"), **a)
+    assert not bs.calls and not vs.calls
+    vs.sample_hidden(StandInHead("cuda:0"), **a)
+    assert len(vs.calls) == 1
+
+
+def test_sample_hidden_has_a_buffer_for_every_row(built_lib):
+    import torch
+    bs, head = sampler_without_a_gpu(), StandInHead("cuda:0")
+    whole = hidden_args()
+    for name, t in whole.items():
+        if name == "hidden":
+            continue
+        short = torch.empty((t.shape[0] - 1, *t.shape[1:]), dtype=t.dtype, device="meta")
+        refused(f"{name}: fewer than 3 rows", bs.sample_hidden, head, **{**whole, name: short})
+    assert not bs.calls
+    bs.sample_hidden(head, **whole)
+    for name in ("hist", "hist_len", "probs", "status"):
+        bs.sample_hidden(head, **{**whole, name: None})
+    assert len(bs.calls) == 5 and bs.calls[0][1]["rows"] == 3
