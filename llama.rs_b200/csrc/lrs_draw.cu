@@ -25,6 +25,7 @@
 // 17 operations an element of a pipe of half rate, and the levels' additions to shared memory fill the SMs.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -277,6 +278,7 @@ struct Args {
     int32_t* status;
     uint32_t n;
     uint32_t twice;  // rows, where the grid goes over them twice (0: once)
+    uint32_t most, fill;  // guess_for()
 };
 
 // The row as this call sees it: element i at base[i + skew], base on a 16-byte boundary.
@@ -1049,14 +1051,14 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
         const uint32_t unit = min(mass_unit(chunks), 1u << 24);
         const uint64_t mass_goal = by_mass ? __double2ull_ru(fmin(reach_hi * unit, 0x1p40)) : ~0ull;
         Bound bound{top, low < top ? fminf(255.9f / (0.5f * top - 0.5f * low), 0x1p100f) : 1.0f, 0.0f, 1e30f};  // (halves: no overflow)
-        // Where they do not fill either, a bound at 4.5 % of the maxima from below leaves about 3.1 elements a
-        // chunk of 128 above it (3,700 at n = 151,936), whatever the values if they come in no order: a list that may
-        // do, and shows it if it does.  It is tried where k is that small, or the mass above the bound seems to
+        // Where they do not fill either, the bound goes down to where the list is as good as full, g.most maxima
+        // (guess_for()), whatever the values if they come in no order: a list that may do, and shows it if it
+        // does.  It is tried where k is at most what it then holds, g.fill, or the mass above the bound seems to
         // be enough: if a share 1 - i / N of the chunks has nothing above x, -ln(1 - i / N) elements a chunk lie
         // there, so that the i-th largest maximum stands for N / (N - i) elements.  "Enough" begins at 0.96 of the
         // goal: at 0.90 rows whose nucleus is a little too long listed in vain (1,024 x 151,936, sigma 3, top_p 0.9 in
         // 842 us, 670 at 0.98), at 0.98 rows that would do went on (Zipf-like, top_p 0.85-0.95: 272 us, 199 at 0.94).
-        const uint32_t most = (uint32_t)(n / kChunk * 0.955f);
+        const uint32_t most = g.most;
         bool guess = false, bounded = true;
         uint32_t reaching = 0;
         for (int round = 0; round < 2; ++round) {
@@ -1089,7 +1091,7 @@ __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
                 const uint32_t edge = block_min(upto >= most ? bin : kAll, sh);
                 Sum held{0, 0.0, 0.0};
                 if (bin <= edge) held.lo = few_w[bin] * ((double)chunks / (chunks - min(before_n + few_n[bin] / 2, chunks - 1)));
-                guess = k <= kList * 7 / 8 || (by_mass && block_scan(held, nullptr, sh).lo >= 0.96 * (double)mass_goal);
+                guess = k <= g.fill || (by_mass && block_scan(held, nullptr, sh).lo >= 0.96 * (double)mass_goal);
                 if (guess) at = edge;
             }
             if (at == kAll) {  // not even all of them: every element from `least` up
@@ -1564,6 +1566,36 @@ size_t shared_bytes(uint32_t n) {
     return kList * 8 + kChunks * 4 + kSlots * 16 + (tiles + 1) / 2 * 2 * 8 + (size_t)tiles * kPer * 4;
 }
 
+// The guessed list of rows of n elements: `most`, how many of the N chunk maxima it takes in, and `fill`, how many
+// elements it then holds more often than not.  With j maxima left below the bound, the elements above it are N times the
+// (j + 1)-th smallest of N exponential variables turned over: N ln((N + 1/2) / (j + 1/2)) of them, N / sqrt(j + 0.6) their
+// standard deviation.  j is the least that leaves two and a half of those to the list's end (a row in a hundred overflows at
+// most), has its chunks listed, and is 4.5 % of N: longer lists make short rows' nuclei slower (256 x 32,003, 532 kept: 34.9 us,
+// 40.3 with every maximum taken in) and hardly fill more of them.  So 1,133 of 1,187 maxima at n = 151,936, 3,660 +- 160
+// elements; 238 of 250 at 32,003, 750 +- 70; 1,422 of 1,562 at 200,000, 3,760 +- 130.  Sizes that the list does not hold
+// are not guessed (48 x 32,003 fp16, k = 1,000: 43.0 us, 52.3 guessed in vain; 256 x 65,000, k = 2,500: 106 and 126), and long rows'
+// lists no longer overflow, as at 4.5 % alone they did from 169,000 on (256 x 200,000, k = 2,000: 124 us, was 379; 3,060 kept by
+// top-p: 270, was 302).  `fill` is half a deviation below the mean: at 0.6 the last k that gains was lost (1,024 x 151,936,
+// k = 3,570: 672 us guessed, 806 not), at 2 batches of one wave won what those of several lost (k = 3,500: 256 rows 278 -> 258,
+// 1,024 rows 565 -> 805).
+void guess_for(uint32_t n, uint32_t* most, uint32_t* fill) {
+    const uint32_t all = n / kChunk;
+    *most = *fill = 0;
+    if (n <= kList) return;  // (the whole row is listed)
+    auto mean = [&](uint32_t j) { return all * std::log((all + 0.5f) / (j + 0.5f)); };
+    auto deviation = [&](uint32_t j) { return all / std::sqrt(j + 0.6f); };
+    uint32_t j = std::max((uint32_t)std::ceil(all * 0.045f), all > kChunks - 64 ? all - (kChunks - 64) : 0), end = all - 1;
+    while (j < end) {
+        const uint32_t mid = (j + end) / 2;
+        if (mean(mid) + 2.5f * deviation(mid) <= (float)kList)
+            end = mid;
+        else
+            j = mid + 1;
+    }
+    *most = all - j;
+    *fill = (uint32_t)std::fmax(0.0f, mean(j) - 0.5f * deviation(j));
+}
+
 template <typename T>
 int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     int dev = 0;
@@ -1593,6 +1625,9 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     const bool waves = ctas == 1 && rows > 3 * (uint32_t)sms[dev].load();
     Args args = g;
     args.twice = waves ? rows : 0;
+    static thread_local uint32_t known[3];  // n, most, fill of the thread's last call (0.4 us)
+    if (known[0] != g.n) guess_for(g.n, &known[1], &known[2]), known[0] = g.n;
+    args.most = known[1], args.fill = known[2];
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(waves ? 2 * rows : rows * ctas);
     cfg.blockDim = dim3(kThreads);
@@ -1625,7 +1660,7 @@ extern "C" int lrs_draw_device(const void* d_logits, int dtype, uint32_t rows, u
     if ((uintptr_t)d_logits % size || (uintptr_t)d_params % 4 || (uintptr_t)d_uniform % 4 || (uintptr_t)d_tokens % 4 ||
         (uintptr_t)d_probs % 4 || (uintptr_t)d_kept % 4 || (uintptr_t)d_status % 4)
         return lrs_call_error(LRS_E_INVALID, "lrs_draw_device: a buffer is not aligned to its type");
-    const Args g{d_logits, ld, d_params, d_uniform, d_tokens, d_probs, d_kept, d_status, n, 0};
+    const Args g{d_logits, ld, d_params, d_uniform, d_tokens, d_probs, d_kept, d_status, n, 0, 0, 0};
     const cudaStream_t s = (cudaStream_t)stream;
     return dtype == LRS_F32 ? launch<float>(g, rows, s) : dtype == LRS_BF16 ? launch<__nv_bfloat16>(g, rows, s) : launch<__half>(g, rows, s);
 }

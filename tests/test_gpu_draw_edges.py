@@ -81,3 +81,25 @@ def test_a_cut_among_masses_below_the_histograms_unit(rows):
     u[:2] = 0.0, 1 - 2.0 ** -24
     got = run(torch.from_numpy(x[None]).cuda(), params, u, ld=0)
     check(got, [x.astype(np.float64)] * rows, params, u)
+
+
+@pytest.mark.parametrize("n", [4097, 8000, 32003, 65000, 200000, 400001])
+def test_lists_as_long_as_they_may_be(n):
+    """Cuts at and around what a guessed list holds at each length (fill), up to the list's end and past it, in rows
+    of random and of sorted order (where a guess made from the chunks' maxima is wrong) and with closed elements."""
+    import torch
+    rng = np.random.default_rng([17, n])
+    fill = {4097: 72, 8000: 162, 32003: 714, 65000: 1505, 200000: 3696, 400001: 3101}[n]
+    x = rng.standard_normal((12, n)) * 3
+    x[1::4] = np.sort(x[1::4])[:, ::-1]
+    x[2::4][rng.random((3, n)) < 0.5] = -np.inf
+    x[3::4, ::128] = np.sort(x[3::4, ::128]) + 9.0  # (every chunk's maximum far above its other elements)
+    x = x.astype(np.float32)
+    t, want = torch.from_numpy(x).cuda(), x.astype(np.float64)
+    reach = np.cumsum(np.sort(np.exp(want[0] - want[0].max()))[::-1])
+    mass = [float(reach[c - 1] / reach[-1]) for c in (fill // 2, fill - 1, fill + 1, min(n - 1, 3900))]  # (nuclei of so many)
+    filters = [(1.0, k, 1.0, 0.0) for k in (fill - 1, fill, fill + 1, min(4096, n), min(4097, n))]
+    filters += [(1.0, 0, p, 0.0) for p in mass] + [(1.0, fill, mass[2], 0.0), (1.0, fill + 50, mass[1], 1e-9)]
+    for shift in range(len(filters)):
+        params, u = records(12, filters[shift:] + filters[:shift]), rng.random(12, np.float32)
+        check(run(t, params, u), want, params, u, shift)
