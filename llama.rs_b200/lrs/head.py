@@ -13,7 +13,7 @@ cudaStream_t handle of that device) where one is given.
 """
 from __future__ import annotations
 
-from .sampler import LRS_E_INVALID, SamplerError, check_kind, dtype_code, launch, lib
+from .sampler import LRS_E_INVALID, SamplerError, check_kind, dtype_code, kinds, launch, lib
 
 BLOCK = 128
 
@@ -23,7 +23,7 @@ def _matrix(t, rows: int, cols: int, kind, what: str) -> int:
     caller has looked); rows of one have none."""
     if t.shape != (rows, cols):
         raise SamplerError(LRS_E_INVALID, f"{what}: a tensor of {rows} x {cols} is needed")
-    if kind is not None:
+    if kind and t.dtype not in kinds[kind]:
         check_kind(t, kind, what)
     step, inner = t.stride()
     if inner != 1 and cols > 1:
@@ -36,12 +36,12 @@ def _blocks(k: int) -> int:
 
 
 def _two(t, what: str):
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise SamplerError(LRS_E_INVALID, f"{what}: a 2-d tensor is needed")
-    rows, cols = t.shape
-    if rows >> 32 or cols >> 32:  # (ctypes would cut them)
-        raise SamplerError(LRS_E_INVALID, f"{what}: {rows} x {cols} is larger than 2^32 a side")
-    return rows, cols
+    if (shape[0] | shape[1]) >> 32:  # (ctypes would cut them)
+        raise SamplerError(LRS_E_INVALID, f"{what}: {shape[0]} x {shape[1]} is larger than 2^32 a side")
+    return shape
 
 
 def _quantize(call, x, codes, scales, a: int, b: int, stream) -> None:

@@ -153,7 +153,7 @@ def _check(code: int, ctx=None):
 
 
 _dtype_codes = None
-_kinds: dict = {}
+kinds: dict = {"codes": (), "f32": (), "i32": ()}  # of types (check_kind fills them)
 
 
 def dtype_code(t) -> int:
@@ -170,10 +170,10 @@ def dtype_code(t) -> int:
 
 def check_kind(t, kind: str, what: str) -> None:
     """Refuses a tensor whose type is not of a kind: "codes" (e4m3 values or their bytes), "f32" or "i32"."""
-    if not _kinds:
+    if not kinds[kind]:
         import torch
-        _kinds.update(codes={torch.float8_e4m3fn, torch.uint8}, f32={torch.float32}, i32={torch.int32, torch.uint32})
-    if t.dtype not in _kinds[kind]:
+        kinds.update(codes={torch.float8_e4m3fn, torch.uint8}, f32={torch.float32}, i32={torch.int32, torch.uint32})
+    if t.dtype not in kinds[kind]:
         names = {"codes": "float8_e4m3fn or uint8", "f32": "float32", "i32": "int32"}
         raise SamplerError(LRS_E_INVALID, f"{what}: {t.dtype}, {names[kind]} is needed")
 
@@ -335,17 +335,19 @@ class BatchSampler:
         if inner != 1 and width > 1:
             raise SamplerError(LRS_E_INVALID, "logits: a 2-d tensor with contiguous rows is needed")
         n = width if n is None else n
+        if (rows | n) >> 32:  # (ctypes would cut them)
+            raise SamplerError(LRS_E_INVALID, f"draw_device: {rows} rows of {n}")
         if ld is None:
             ld = step if have > 1 else n if rows <= 1 else 0
-        # (sizes that ctypes would cut to 32 bits, and a given ld that leads past the tensor's last element)
-        if rows >> 32 or n >> 32 or ld < 0 or (rows > 1 and (rows - 1) * ld + n > (have - 1) * step + width):
+        elif ld < 0 or (rows > 1 and (rows - 1) * ld + n > (have - 1) * step + width):
             raise SamplerError(LRS_E_INVALID, f"draw_device: {rows} rows of {n}, {ld} apart, do not lie within the logits")
         if (rows > have and ld) or n > width or params.numel() * params.element_size() < 16 * rows:
             raise SamplerError(LRS_E_INVALID, f"draw_device: the logits or the parameters hold fewer than {rows} rows of {n}")
         for t, kind, what in ((uniform, "f32", "uniform"), (tokens, "i32", "tokens"), (probs, "f32", "probs"),
                               (kept, "i32", "kept"), (status, "i32", "status")):
             if t is not None:
-                check_kind(t, kind, what)
+                if t.dtype not in kinds[kind]:
+                    check_kind(t, kind, what)
                 if t.numel() < rows or not t.is_contiguous():
                     raise SamplerError(LRS_E_INVALID, f"{what}: not {rows} values in a row")
         if not params.is_contiguous():
