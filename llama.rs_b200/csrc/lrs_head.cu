@@ -6,7 +6,7 @@
 // fills another TMEM buffer.  Persistent CTAs: warp 0 issues the TMA copies of both operands
 // (128-byte swizzle, a ring of stages), 1 issues the MMAs, the last 16 are the epilogue.  Tiles walk the row
 // tiles first, so that the CTAs share the weights they stream in L2.  Two forms:
-//   narrow  up to 64 rows (a decode step; bound by the weights' bytes): the weights are the tensor core's
+//   narrow  up to 32 or 64 rows (a decode step; bound by the weights' bytes): the weights are the tensor core's
 //           128-row operand, so a few rows cost a narrow instruction and not a padded one, and a warp's
 //           lanes are consecutive logits of one row.  A row is a TMEM column there, its scale the same
 //           for a whole warp: warp 2 brings them to shared memory (4-byte asynchronous copies: any
@@ -30,7 +30,12 @@ namespace {
 using namespace lrs;
 
 constexpr uint32_t kBlock = 128;      // columns a scale covers, and columns of a step
-constexpr uint32_t kNarrowRows = 64;  // rows of the narrow form at most
+// Rows of the narrow form at most, and where rows of d_out start on 16-byte boundaries (the wide form stores others element by
+// element).  Measured, narrow and wide, us (one B200): 151,936 x 4,096 bf16 17 rows 108.7 and 134.0, 32 rows 109.6 and 111.3,
+// 48 rows 135.5 and 113.4, 64 rows 138.6 and 115.7, 65 rows (two narrow tiles) 258 and 113; 151,936 x 1,024 f32 32 rows 33.9 and 38.0, 64
+// rows 40.3 and 41.1, 65 rows 72.0 and 41.2; 32,000 x 2,048 f32 32 rows 16.1 and 15.5, 64 rows 20.1 and 13.6.  Unaligned, 109,051 x
+// 2,048 bf16: 32 rows 43.4 and 55.1, 64 rows 50.6 and 52.5, 65 rows 96.2 and 52.7.
+constexpr uint32_t kNarrowRows = 64, kNarrowAligned = 32;
 constexpr uint32_t kThreads = 640;  // of both forms
 constexpr uint32_t kMaxBuffers = 8;   // TMEM accumulators
 constexpr uint32_t kScaleStages = 8;
@@ -566,7 +571,8 @@ int launch(void (*kernel)(CUtensorMap, CUtensorMap, Args), DeviceInfo* info, con
 template <typename T>
 int run(const uint8_t* d_a, uint64_t ld_a, const uint8_t* d_w, uint64_t ld_w, uint32_t k, Args g, cudaStream_t s) {
     static DeviceInfo narrow_info[kMaxDevices], wide_info[kMaxDevices];
-    const bool narrow = g.rows <= kNarrowRows;
+    g.wide_out = (uintptr_t)g.out % 16 == 0 && (g.rows == 1 || g.ld_out * sizeof(T) % 16 == 0);
+    const bool narrow = g.rows <= (g.wide_out ? kNarrowAligned : kNarrowRows);
     g.tile_r = narrow ? (g.rows + 15) / 16 * 16 : kWideR;
     g.tile_v = narrow ? 128 : kWideV;
     g.row_tiles = (g.rows + g.tile_r - 1) / g.tile_r;
@@ -579,7 +585,6 @@ int run(const uint8_t* d_a, uint64_t ld_a, const uint8_t* d_w, uint64_t ld_w, ui
     g.buffers = 512 / g.columns < kMaxBuffers ? 512 / g.columns : kMaxBuffers;
     g.tmem_columns = 32;
     while (g.tmem_columns < g.buffers * g.columns) g.tmem_columns *= 2;
-    g.wide_out = (uintptr_t)g.out % 16 == 0 && (g.rows == 1 || g.ld_out * sizeof(T) % 16 == 0);
     CUtensorMap ma, mw;
     if (!code_map(&mw, d_w, g.n, k, ld_w, g.tile_v) || !code_map(&ma, d_a, g.rows, k, ld_a, g.tile_r))
         return lrs_call_error(LRS_E_INVALID, "lrs_fp8_logits: the codes cannot be mapped (ld too large?)");
