@@ -18,17 +18,22 @@ from .sampler import LRS_E_INVALID, SamplerError, check_kind, dtype_code, kinds,
 BLOCK = 128
 
 
-def _matrix(t, rows: int, cols: int, kind, what: str) -> int:
-    """The leading dimension of a rows x cols tensor of contiguous rows and a kind of type (check_kind; None: the
-    caller has looked); rows of one have none."""
-    if t.shape != (rows, cols):
-        raise SamplerError(LRS_E_INVALID, f"{what}: a tensor of {rows} x {cols} is needed")
+def _lead(t, rows: int, cols: int, kind, what: str) -> int:
+    """The leading dimension of a rows x cols tensor of contiguous rows (rows of one have none) and a kind of type
+    (check_kind; None: the caller has looked)."""
     if kind and t.dtype not in kinds[kind]:
         check_kind(t, kind, what)
     step, inner = t.stride()
     if inner != 1 and cols > 1:
         raise SamplerError(LRS_E_INVALID, f"{what}: contiguous rows are needed")
     return step if rows > 1 else cols
+
+
+def _matrix(t, rows: int, cols: int, kind, what: str) -> int:
+    """_lead() of a tensor that has to be rows x cols."""
+    if t.shape != (rows, cols):
+        raise SamplerError(LRS_E_INVALID, f"{what}: a tensor of {rows} x {cols} is needed")
+    return _lead(t, rows, cols, kind, what)
 
 
 def _blocks(k: int) -> int:
@@ -47,7 +52,7 @@ def _two(t, what: str):
 def _quantize(call, x, codes, scales, a: int, b: int, stream) -> None:
     rows, k = x.shape
     launch(call, stream,
-           (x.data_ptr(), dtype_code(x), rows, k, _matrix(x, rows, k, None, "x"), codes.data_ptr(),
+           (x.data_ptr(), dtype_code(x), rows, k, _lead(x, rows, k, None, "x"), codes.data_ptr(),
             _matrix(codes, rows, k, "codes", "codes"), scales.data_ptr(), _matrix(scales, a, b, "f32", "scales")),
            x, codes, scales)
 
@@ -70,7 +75,7 @@ def quantize_blocks(x, codes, scales, stream=None) -> None:
 def _product(a, a_scales, w, w_scales, out) -> tuple:
     rows, k = _two(a, "a")
     n, kb = _two(w, "w")[0], _blocks(k)
-    return (a.data_ptr(), _matrix(a, rows, k, "codes", "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, "f32", "a_scales"),
+    return (a.data_ptr(), _lead(a, rows, k, "codes", "a"), a_scales.data_ptr(), _matrix(a_scales, kb, rows, "f32", "a_scales"),
             w.data_ptr(), _matrix(w, n, k, "codes", "w"), w_scales.data_ptr(), _matrix(w_scales, _blocks(n), kb, "f32", "w_scales"),
             rows, n, k, out.data_ptr(), dtype_code(out), _matrix(out, rows, n, None, "out"))
 

@@ -178,6 +178,15 @@ def check_kind(t, kind: str, what: str) -> None:
         raise SamplerError(LRS_E_INVALID, f"{what}: {t.dtype}, {names[kind]} is needed")
 
 
+def check_buffers(rows: int, **buffers) -> None:
+    """Refuses by its name a buffer (None: absent) that is not `rows` values in a row of its type."""
+    for what, t in buffers.items():
+        if t is not None:
+            check_kind(t, "f32" if what in ("uniform", "probs") else "i32", what)
+            if t.numel() < rows or not t.is_contiguous():
+                raise SamplerError(LRS_E_INVALID, f"{what}: not {rows} values in a row")
+
+
 _raw_stream = _raw_device = None
 
 
@@ -343,13 +352,11 @@ class BatchSampler:
             raise SamplerError(LRS_E_INVALID, f"draw_device: {rows} rows of {n}, {ld} apart, do not lie within the logits")
         if (rows > have and ld) or n > width or params.numel() * params.element_size() < 16 * rows:
             raise SamplerError(LRS_E_INVALID, f"draw_device: the logits or the parameters hold fewer than {rows} rows of {n}")
-        for t, kind, what in ((uniform, "f32", "uniform"), (tokens, "i32", "tokens"), (probs, "f32", "probs"),
-                              (kept, "i32", "kept"), (status, "i32", "status")):
-            if t is not None:
-                if t.dtype not in kinds[kind]:
-                    check_kind(t, kind, what)
-                if t.numel() < rows or not t.is_contiguous():
-                    raise SamplerError(LRS_E_INVALID, f"{what}: not {rows} values in a row")
+        f32, i32 = kinds["f32"], kinds["i32"]
+        for t, types in ((uniform, f32), (tokens, i32), (probs, f32), (kept, i32), (status, i32)):
+            if t is not None and (t.dtype not in types or t.numel() < rows or not t.is_contiguous()):
+                check_buffers(rows, uniform=uniform, tokens=tokens, probs=probs, kept=kept, status=status)
+                break
         if not params.is_contiguous():
             raise SamplerError(LRS_E_INVALID, "draw_device: the parameters are not contiguous")
         launch(lib().lrs_draw_device, stream,
