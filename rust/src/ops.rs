@@ -137,12 +137,19 @@ pub unsafe fn quantize(x: Matrix, dtype: Dtype, tall: bool, d_q: *mut u8, ld_q: 
     )
 }
 
-/// The head's product of codes, out.rows x out.cols (lrs_fp8_logits).
+/// The head's product of codes, out.rows x out.cols (lrs_fp8_logits); matrices whose sizes do not agree are
+/// refused (LRS_E_INVALID).
 ///
 /// # Safety
 /// Device pointers of the sizes the C header gives, on the current device.
 pub unsafe fn fp8_logits(a: Matrix, d_a_scale: *const f32, ld_as: u64, w: Matrix, d_w_scale: *const f32, ld_ws: u64,
                          out: Matrix, out_dtype: Dtype, stream: *mut c_void) -> Result<(), SamplerError> {
+    if w.cols != a.cols || out.rows != a.rows || out.cols != w.rows {
+        return Err(SamplerError {
+            code: ffi::LRS_E_INVALID,
+            message: format!("fp8_logits: {} x {} times {} x {} into {} x {}", a.rows, a.cols, w.rows, w.cols, out.rows, out.cols),
+        });
+    }
     check(
         lrs_fp8_logits(a.data as *const u8, a.ld, d_a_scale, ld_as, w.data as *const u8, w.ld, d_w_scale, ld_ws, a.rows,
                        w.rows, a.cols, out.data, out_dtype as c_int, out.ld, stream),

@@ -194,3 +194,13 @@ def test_sample_hidden_has_a_buffer_for_every_row(built_lib):
     for name in ("hist", "hist_len", "probs", "status"):
         bs.sample_hidden(head, **{**whole, name: None})
     assert len(bs.calls) == 5 and bs.calls[0][1]["rows"] == 3
+
+
+def test_the_crates_product_compares_every_size_of_its_matrices():
+    """rust/src/ops.rs is not compiled here: the sizes that its safe types carry and the C call does not are looked
+    for in its text (w.cols, out.rows, out.cols went unread)."""
+    import os
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rust", "src", "ops.rs")).read()
+    body = text[text.index("pub unsafe fn fp8_logits("):]
+    guard = body[:body.index("lrs_fp8_logits(")]
+    assert "if w.cols != a.cols || out.rows != a.rows || out.cols != w.rows {" in guard and "ffi::LRS_E_INVALID" in guard
