@@ -292,8 +292,8 @@ int  lrs_draw_device(const void* d_logits, int dtype, uint32_t rows, uint32_t n,
  *   ld_q bytes (ld_q >= k); bytes k .. ld_q of a row are left as they were.
  * lrs_fp8_logits       d_out[r][v] = sum over b of a_scale[b * ld_as + r] * w_scale[v / 128 * ld_ws + b]
  *                      * (sum over the block's columns of a[r][c] * w[v][c]), r < rows, v < n: the
- *                      block sums in f32 on the tensor cores, the sum over blocks in f32, rounded
- *                      once to out_dtype.  d_out: row r at d_out + r * ld_out elements (ld_out >=
+ *                      block sums in f32 on the tensor cores, the scales' product first, in f32 (so
+ *                      it has to be finite), the sum over blocks in f32, rounded once to out_dtype.  d_out: row r at d_out + r * ld_out elements (ld_out >=
  *                      n, any alignment of the type).  Codes: d_a + r * ld_a and d_w + v * ld_w
  *                      bytes (>= k), bases and (of more than one row) ld_a, ld_w multiples of 16.
  *                      A tile whose bounded waits ran out (about 2 s; none does in a sound launch) is NaN.

@@ -20,9 +20,10 @@
 //      pass sums what lies above it by tile and lists the bracket, and the token is found by tile,
 //      then inside one tile.  Without any filter step 1 sums in 64 bits and goes there directly.
 // Measured (one B200, passes over changing inputs, f32 rows of 151,936): one row under the default filters 16.4 us, a
-// chain of short stages after a pass of 4 us; 1,024 rows under mixed filters 192 us (their bytes alone: 95); 512 rows
-// with nuclei of 12,000 to 119,000 tokens 415 us (48), where step 3 reads the row twice more and the 64-bit powers,
-// 17 operations an element of a pipe of half rate, and the levels' additions to shared memory fill the SMs.
+// chain of short stages after a pass of 4 us; 1,024 rows under mixed filters 160 to 215 us (their bytes alone: 95), by
+// the inputs: a row with a large nucleus has one CTA and reads its logits three times, and the batch waits for the last
+// such row; 512 rows with nuclei of 12,000 to 119,000 tokens 415 us (48), where step 3 reads the row twice more and the
+// 64-bit powers, 17 operations an element of a pipe of half rate, and the levels' additions to shared memory fill the SMs.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -851,6 +852,10 @@ __device__ __noinline__ Cut find_cut(uint64_t* list, uint32_t* slots, uint32_t* 
     return Cut{keep ? list[keep - 1] : ~0ull, keep, keep == keep_hi, true};
 }
 
+// Three CTAs an SM leave 80 registers, of which some 800 bytes a thread are spilled over the kernel; two leave 128 and 48
+// bytes.  Three and two, us (one B200, f32 rows of 151,936, graph replays over three inputs): 1,024 mixed 162 and 184, 1,024
+// default filters 160 and 182, 1,024 unfiltered 236 and 270, 512 large nuclei 416 and 384, 256 x 109,051 bf16 min-p 50.6 and 48.6,
+// one row 15.4 and 14.6: batches of several waves need the third, the others lose 4 to 8 % by it.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const Args g) {
     extern __shared__ __align__(16) uint8_t dynamic[];
@@ -1620,8 +1625,10 @@ int launch(const Args& g, uint32_t rows, cudaStream_t s) {
     uint32_t ctas = 1;
     while (ctas < kMaxCluster && (uint64_t)rows * ctas * 2 <= 2 * (uint64_t)sms[dev].load() && ctas * kWarps < tiles) ctas *= 2;
     // Batches of several waves go over the rows twice, the heavy rows first, so that no such row is among the last
-    // to start: 1,024 x 151,936 with mixed filters in 162 us and not 193.  The CTAs that find their row in the other
-    // half leave at once.  (With one wave all start together: the second half would only cost.)
+    // to start: 1,024 x 151,936 with mixed filters in 162 us and not 193 (graph replays on one input).  The CTAs that find
+    // their row in the other half leave at once.  (With one wave all start together: the second half would only cost.  Three
+    // CTAs an SM hold up to n = 640,000; of longer rows, whose maxima and sums take more shared memory, a wave is smaller, and
+    // batches of 149 or 297 rows up to three an SM keep the order of their rows.)
     const bool waves = ctas == 1 && rows > 3 * (uint32_t)sms[dev].load();
     Args args = g;
     args.twice = waves ? rows : 0;

@@ -99,7 +99,8 @@ def empty_codes(rows: int, k: int, device):
 
 
 class LmHead:
-    """A head's weights (vocab, k), quantised once to e4m3 with a scale per 128 x 128 block."""
+    """A head's weights (vocab, k), quantised once to e4m3 with a scale per 128 x 128 block, on torch's current stream of
+    their device: a product on another stream has to be ordered after that one, as any tensor's first use is."""
 
     def __init__(self, weight):
         import torch
