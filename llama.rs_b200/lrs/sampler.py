@@ -379,17 +379,24 @@ class BatchSampler:
         if head.device.type != "cuda" or head.device.index != self.device:
             raise SamplerError(LRS_E_INVALID, f"the head lies on {head.device}, the sampler on cuda:{self.device}")
 
+    def check_rows(self, rows: int, **buffers) -> None:
+        """Refuses by its name a buffer of sample_device (None: absent) that does not lie on the sampler's GPU or holds
+        fewer than `rows` rows."""
+        size = {"params": PARAMS_DTYPE.itemsize, "state": 8}
+        for what, t in buffers.items():
+            if t is None:
+                continue
+            if t.is_cpu or (t.is_cuda and t.get_device() != self.device):
+                raise SamplerError(LRS_E_INVALID, f"{what}: not on cuda:{self.device}")
+            if (t.shape[0] if what == "hist" else t.numel() * t.element_size() // size.get(what, 4)) < rows:
+                raise SamplerError(LRS_E_INVALID, f"{what}: fewer than {rows} rows")
+
     def sample_hidden(self, head, hidden, params, state, tokens, hist=None, hist_len=None, probs=None, status=None):
         """The same with the exact sampler: the head's logits of the hidden states, then sample_device.  The head lies
         on the sampler's device, and every buffer holds a row for each hidden state."""
         self.check_head(head)
         rows = hidden.shape[0]
-        for t, size, what in ((params, PARAMS_DTYPE.itemsize, "params"), (state, 8, "state"), (tokens, 4, "tokens"),
-                              (hist_len, 4, "hist_len"), (probs, 4, "probs"), (status, 4, "status")):
-            if t is not None and t.numel() * t.element_size() < size * rows:
-                raise SamplerError(LRS_E_INVALID, f"{what}: fewer than {rows} rows")
-        if hist is not None and hist.shape[0] < rows:
-            raise SamplerError(LRS_E_INVALID, f"hist: fewer than {rows} rows")
+        self.check_rows(rows, params=params, state=state, tokens=tokens, hist=hist, hist_len=hist_len, probs=probs, status=status)
         logits = head.logits(hidden)
         self.sample_device(logits, params, state, tokens, hist=hist, hist_len=hist_len, probs=probs, status=status, rows=rows)
         return logits

@@ -215,6 +215,7 @@ class VocabShardedSampler:
         if head.vocab != self.shard_n or hidden.shape[0] != self.rows:
             raise ValueError(f"a head of {self.shard_n} tokens and {self.rows} hidden states are needed")
         self.bs.check_head(head)
+        self.bs.check_rows(self.rows, params=params, hist=hist, hist_len=hist_len)
         self.sample(head.logits(hidden), params, state, tokens, hist=hist, hist_len=hist_len, probs=probs,
                     status=status)
 

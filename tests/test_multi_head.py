@@ -53,6 +53,7 @@ def _worker(rank, world, port, out_dir):
                 self.rows, self.shard_n = ROWS, VOCAB // world
                 self.bs = BatchSampler.__new__(BatchSampler)
                 self.bs._h, self.bs.device = None, 0
+                self.bs.check_rows = lambda rows, **buffers: None  # (they lie on the host here)
 
             def sample(self, shard, params, state, tokens, hist=None, hist_len=None, probs=None, status=None, stream=None):
                 full = S.owner_exchange_host(shard.numpy(), ROWS)

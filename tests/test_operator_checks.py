@@ -196,6 +196,24 @@ def test_sample_hidden_has_a_buffer_for_every_row(built_lib):
     assert len(bs.calls) == 5 and bs.calls[0][1]["rows"] == 3
 
 
+def test_sample_hiddens_buffers_lie_on_the_gpu(built_lib):
+    """Their addresses go to the kernels as they are."""
+    import torch
+    from lrs.sharded import VocabShardedSampler
+    bs, head = sampler_without_a_gpu(), StandInHead("cuda:0")
+    vs = VocabShardedSampler.__new__(VocabShardedSampler)
+    vs.shard_n, vs.rows, vs.bs = 5, 3, bs
+    vs.sample = lambda *args, **kw: bs.calls.append((args, kw))
+    whole = hidden_args()
+    for name, t in whole.items():
+        host = {**whole, name: torch.zeros(t.shape, dtype=t.dtype)}
+        if name != "hidden":  # (LmHead.logits refuses those)
+            refused(f"{name}: not on cuda:0", bs.sample_hidden, head, **host)
+        if name in ("params", "hist", "hist_len"):  # (the others are copied by torch there)
+            refused(f"{name}: not on cuda:0", vs.sample_hidden, head, **host)
+    assert not bs.calls
+
+
 def test_the_crates_product_compares_every_size_of_its_matrices():
     """rust/src/ops.rs is not compiled here: the sizes that its safe types carry and the C call does not are looked
     for in its text (w.cols, out.rows, out.cols went unread)."""
