@@ -21,8 +21,8 @@
 //      then inside one tile.  Without any filter step 1 sums in 64 bits and goes there directly.
 // Measured (one B200, passes over changing inputs, f32 rows of 151,936): one row under the default filters 16.4 us, a
 // chain of short stages after a pass of 4 us; 1,024 rows under mixed filters 160 to 275 us (199 on average over 24
-// inputs; their bytes alone: 95): a row with a large nucleus has one CTA and reads its logits three times, and the batch waits for the last
-// such row; 512 rows with nuclei of 12,000 to 119,000 tokens 415 us (48), where step 3 reads the row twice more and the
+// inputs; their bytes alone: 95): a row with a large nucleus has one CTA and reads its logits three times, and the batch
+// waits for the last such row; 512 rows with nuclei of 12,000 to 119,000 tokens 415 us (48), where step 3 reads the row twice more and the
 // 64-bit powers, 17 operations an element of a pipe of half rate, and the levels' additions to shared memory fill the SMs.
 #include <cooperative_groups.h>
 

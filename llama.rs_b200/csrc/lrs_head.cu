@@ -16,10 +16,11 @@
 //           columns the scales' shared-memory reads and products took three times the MMAs' time); the
 //           logits go out through shared memory, 64 bytes of a row at a time.
 // Measured (one B200): 1 x 151,936 x 1,024 in 31.8 us (5.0 TB/s); n = 109,051, k = 2,048, bf16 over changing inputs: 1 to 32
-// rows in 45 to 47 us (4.9 to 5.0 TB/s, three quarters of the copy rate: the weights' way in), 64 rows in 51 to 55 us (4.4 to 4.7), where
-// the epilogue's reads of TMEM and the activations' codes, fetched again for every tile, add to it; 256 x 151,936 x 4,096 f32 in 189 us and 1,024 in 650-680 us (1.9 PFLOP/s; 799 under the power cap),
-// bound by the block sums' way through the epilogue warps (tensor pipe 48 % busy).  Rows on no 16-byte boundary cost
-// the wide form 40 % (237 x 109,051 x 1,000 f32: 79 us and not 56).
+// rows in 45 to 47 us (4.9 to 5.0 TB/s, three quarters of the copy rate: the weights' way in), 64 rows in 51 to 59 us (4.0 to
+// 4.7), where the epilogue's reads of TMEM and the activations' codes, fetched again for every tile, add to it; 256 x
+// 151,936 x 4,096 f32 in 200 us and 1,024 rows in 650 to 680 us (1.9 PFLOP/s; 781 under the power cap), bound by the block
+// sums' way through the epilogue warps (tensor pipe 48 % busy).  Rows on no 16-byte boundary cost the wide form a third
+// (237 x 109,051 x 1,000: f32 72 us and not 54, bf16 63 and not 47).
 #include <cuda.h>
 
 #include <atomic>
