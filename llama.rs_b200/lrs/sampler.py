@@ -333,7 +333,7 @@ class BatchSampler:
                     ld=None, rows=None):
         """Tokens from given uniforms (lrs_draw_device) under temperature, top-k, top-p and min-p:
         logits (rows, n) float32 / bfloat16 / float16, params rows of DRAW_PARAMS_DTYPE (any 4-byte or
-        byte tensor of them), uniform float32 in [0, 1); tokens, kept and status are int32 tensors,
+        byte tensor of them), uniform float32 in [0, 1); tokens, kept and status are int32 (or uint32) tensors,
         probs float32.  The definition of the kept set and of the draw is the header's.  Async; no
         working memory and no context, so calls may overlap and be captured."""
         rows = tokens.numel() if rows is None else rows
